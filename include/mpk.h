@@ -192,6 +192,80 @@ int mpk_gemm_mxfp8_bf16_gather(const uint8_t* A_data, const uint8_t* A_scales, c
  * the reference. */
 int mpk_peer_barrier(uint32_t* const* flags, int rank, int world, uint32_t epoch, void* stream);
 
+/* Element types of the int8 and expert-grouped entry points below. */
+#define MPK_TYPE_F32 0
+#define MPK_TYPE_BF16 1
+#define MPK_TYPE_F16 2
+/* Storage of B in those entry points: [K][N] as in the GEMM above, or [N][K] (the
+ * reduction contiguous, as a linear layer stores its weight). */
+#define MPK_B_KN 0
+#define MPK_B_NK 1
+/* Most groups of one grouped product. */
+#define MPK_MAX_GROUPS 1024
+
+/* Quantizers to 8-bit integers, x or w of MPK_TYPE_*.  For each row of x [M][K] (rows
+ * ldx elements apart; a token), or each column of w [E][K][N] (rows ldw apart, matrix e
+ * at e * K * ldw; an output channel):
+ *   a = max(max |x|, 2^-100), scale = a / 127, code = rint(x * (127 / a))
+ * in FP32, each operation rounded to nearest (ties to even).  Codes lie in [-127, 127].
+ * A row or column that holds NaN or infinity gets scale NaN and codes 0, so that every
+ * product with it is NaN.  Code rows are ld_codes apart: a multiple of 16 lets the
+ * products read them in place; bytes between K (N) and ld_codes are left as they were.
+ * scales: [M], or [E][N].  No counterpart in the reference. */
+int mpk_int8_quantize_rows(const void* x, int x_type, int64_t ldx, int8_t* codes, int64_t ld_codes,
+                           float* scales, int M, int K, void* stream);
+int mpk_int8_quantize_cols(const void* w, int w_type, int64_t ldw, int8_t* codes, int64_t ld_codes,
+                           float* scales, int E, int K, int N, void* stream);
+
+/* D[m][n] = (sum_k A[m][k] * B[k][n]) * A_scales[m] * B_scales[n] + bias[n]:
+ * the product of int8 codes with one FP32 scale per row of A and per column of B.  The
+ * sum is an exact 32-bit integer (K <= 131071, else MPK_ERR_UNSUPPORTED); it is
+ * converted to FP32, multiplied by the row's and then the column's scale, the bias
+ * (FP32 [N], may be NULL) is added, and the result is rounded once to D's type.
+ * b_layout: MPK_B_KN or MPK_B_NK.  lda, ldb, ldd: row strides in elements.  Any size
+ * and alignment; operands whose base or row stride is not a multiple of 16 bytes are
+ * first copied into a workspace of the library's pool.  No counterpart in the reference. */
+int mpk_gemm_int8(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb, int b_layout,
+                  const float* B_scales, const float* bias, void* D, int d_type, int64_t ldd, int M, int N, int K,
+                  void* stream);
+
+/* mpk_int8_quantize_rows of x, then mpk_gemm_int8: a linear layer with int8 weights and
+ * activations quantized per token.  The codes live in a workspace of the library's pool. */
+int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int64_t ldb, int b_layout,
+                    const float* B_scales, const float* bias, void* D, int d_type, int64_t ldd, int M, int N, int K,
+                    void* stream);
+
+/* Products grouped by expert: rows offsets[e] <= i < offsets[e + 1] of D are the same
+ * rows of A times B[e], e < E.  offsets: int32 [E + 1] in device memory, non-decreasing
+ * (values outside 0..M are clamped to it, a group whose end lies before its start is
+ * empty, and where groups overlap D holds either's rows).  Rows of D outside every group
+ * are left as they were.  B[e] at e * K * ldb (MPK_B_KN) or e * N * ldb (MPK_B_NK); E up to
+ * MPK_MAX_GROUPS.  Nothing is copied to the host: the calls can be captured.
+ *
+ * mpk_gemm_grouped: A and B of the same 16-bit type (MPK_TYPE_BF16 or MPK_TYPE_F16), FP32
+ * sums, D rounded once to d_type.  The gradient of A is the same product of D's gradient
+ * with the same weights in the other layout (N and K swapped).
+ * mpk_gemm_grouped_int8: as mpk_gemm_int8, B_scales [E][N].
+ * mpk_gemm_grouped_mxfp8: A in MXFP8 (codes and scales as in the GEMM above, contiguous),
+ * BF16 B [K][N], D in MXFP8 along N (contiguous).  A is dequantized exactly to BF16 into
+ * a workspace of the library's pool first. */
+int mpk_gemm_grouped(const void* A, int64_t lda, const void* B, int64_t ldb, int b_layout, int ab_type, void* D,
+                     int d_type, int64_t ldd, const int32_t* offsets, int E, int M, int N, int K, void* stream);
+int mpk_gemm_grouped_int8(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb,
+                          int b_layout, const float* B_scales, void* D, int d_type, int64_t ldd,
+                          const int32_t* offsets, int E, int M, int N, int K, void* stream);
+int mpk_gemm_grouped_mxfp8(const uint8_t* A_data, const uint8_t* A_scales, const void* B_bf16, int64_t ldb,
+                           uint8_t* D_data, uint8_t* D_scales, const int32_t* offsets, int E, int M, int N, int K,
+                           void* stream);
+
+/* Gradient of the grouped product's weights: dB[e] = A[rows of e]^T * dD[rows of e], a
+ * K x N matrix (rows ldd apart, matrix e at e * K * ldd) for every e < E; an empty group's
+ * is zeros.  A [M][K] and dD [M][N] of the same 16-bit type, FP32 sums, dB rounded once to
+ * d_type.  offsets as above. */
+int mpk_gemm_grouped_wgrad(const void* A, int64_t lda, const void* dD, int64_t ldg, int ab_type, void* dB,
+                           int d_type, int64_t ldd, const int32_t* offsets, int E, int M, int N, int K,
+                           void* stream);
+
 /* Sharing a device buffer with the other processes of a node (CUDA IPC), for the
  * destinations and flag arrays above.  mpk_ipc_export describes the allocation
  * holding dev_ptr: a 64-byte handle, dev_ptr's offset in it and its size.

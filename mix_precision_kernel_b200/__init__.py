@@ -34,6 +34,11 @@ __all__ = [
     "gemm", "quantize", "dequantize", "device_status", "set_wait_timeout_ns", "wait_selftest",
     "set_gemm_schedule", "gemm_schedule", "gemm_plan", "SCHEDULE_AUTO", "SCHEDULE_TILES", "SCHEDULE_STREAM_K",
     "gemm_path", "PATH_PREPASS", "PATH_ONCHIP",
+    "int8_quantize_rows_gpu", "int8_quantize_cols_gpu", "gemm_int8_gpu", "linear_int8_gpu",
+    "gemm_grouped_gpu", "gemm_grouped_int8_gpu", "gemm_grouped_mxfp8_gpu", "gemm_grouped_wgrad_gpu",
+    "quantize_int8", "quantize_int8_cols", "gemm_int8", "linear_int8",
+    "gemm_grouped", "gemm_grouped_int8", "gemm_grouped_mxfp8", "gemm_grouped_wgrad",
+    "TYPE_F32", "TYPE_BF16", "TYPE_F16", "B_KN", "B_NK", "MAX_GROUPS",
     "MX_BLOCK", "nblk",
 ]
 
@@ -58,6 +63,14 @@ SCHEDULE_STREAM_K = 2
 # Kernel paths of the default GEMM entry point (MPK_PATH_* in include/mpk.h)
 PATH_PREPASS = 0
 PATH_ONCHIP = 1
+# Element types and layouts of B of the int8 and expert-grouped entry points
+# (MPK_TYPE_*, MPK_B_* in include/mpk.h)
+TYPE_F32 = 0
+TYPE_BF16 = 1
+TYPE_F16 = 2
+B_KN = 0
+B_NK = 1
+MAX_GROUPS = 1024
 
 
 class MpkError(RuntimeError):
@@ -119,6 +132,19 @@ def lib() -> ctypes.CDLL:
             ip = ctypes.POINTER(ci)
             L.mpk_gemm_plan.argtypes = [ci, ci, ci, ip, ip, ip]
             L.mpk_gemm_path.argtypes = [vp, vp, ci, ci, ci, ip]
+            i64 = ctypes.c_int64
+            L.mpk_int8_quantize_rows.argtypes = [vp, ci, i64, vp, i64, vp, ci, ci, vp]
+            L.mpk_int8_quantize_cols.argtypes = [vp, ci, i64, vp, i64, vp, ci, ci, ci, vp]
+            L.mpk_gemm_int8.argtypes = [vp, i64, vp, vp, i64, ci, vp, vp, vp, ci, i64, ci, ci, ci, vp]
+            L.mpk_linear_int8.argtypes = [vp, ci, i64, vp, i64, ci, vp, vp, vp, ci, i64, ci, ci, ci, vp]
+            L.mpk_gemm_grouped.argtypes = [vp, i64, vp, i64, ci, ci, vp, ci, i64, vp, ci, ci, ci, ci, vp]
+            L.mpk_gemm_grouped_int8.argtypes = [vp, i64, vp, vp, i64, ci, vp, vp, ci, i64, vp, ci, ci, ci, ci, vp]
+            L.mpk_gemm_grouped_mxfp8.argtypes = [vp, vp, vp, i64, vp, vp, vp, ci, ci, ci, ci, vp]
+            L.mpk_gemm_grouped_wgrad.argtypes = [vp, i64, vp, i64, ci, vp, ci, i64, vp, ci, ci, ci, ci, vp]
+            for f in ("mpk_int8_quantize_rows", "mpk_int8_quantize_cols", "mpk_gemm_int8", "mpk_linear_int8",
+                      "mpk_gemm_grouped", "mpk_gemm_grouped_int8", "mpk_gemm_grouped_mxfp8",
+                      "mpk_gemm_grouped_wgrad"):
+                getattr(L, f).restype = ci
             for f in ("mpk_gemm_mxfp8_bf16", "mpk_gemm_mxfp8_bf16_ws", "mpk_gemm_workspace_size",
                       "mpk_release_workspace_pool", "mpk_mxfp8_quantize", "mpk_mxfp8_dequantize",
                       "mpk_mxfp8_dequantize_bf16", "mpk_gemm_mxfp8_bf16_noalloc",
@@ -377,6 +403,74 @@ def gemm_plan(M: int, N: int, K: int) -> tuple[int, int, int]:
 
 
 # ---------------------------------------------------------------------------
+# int8 and expert-grouped products (tensors or device addresses; see include/mpk.h)
+# ---------------------------------------------------------------------------
+
+def int8_quantize_rows_gpu(input, input_type: int, ld_input: int, codes, ld_codes: int, scales, M: int, K: int,
+                           stream=None) -> None:
+    """int8 codes of input [M, K] and one FP32 scale per row; row strides in elements."""
+    s = _stream(stream, input, codes)
+    _check(lib().mpk_int8_quantize_rows(_addr(input), input_type, ld_input, _addr(codes), ld_codes, _addr(scales),
+                                        M, K, s))
+
+
+def int8_quantize_cols_gpu(input, input_type: int, ld_input: int, codes, ld_codes: int, scales, E: int, K: int,
+                           N: int, stream=None) -> None:
+    """int8 codes of input [E, K, N] and one FP32 scale per matrix and column."""
+    s = _stream(stream, input, codes)
+    _check(lib().mpk_int8_quantize_cols(_addr(input), input_type, ld_input, _addr(codes), ld_codes, _addr(scales),
+                                        E, K, N, s))
+
+
+def gemm_int8_gpu(A, lda: int, A_scales, B, ldb: int, b_layout: int, B_scales, bias, D, d_type: int, ldd: int,
+                  M: int, N: int, K: int, stream=None) -> None:
+    """D = (A*B) * A_scales[row] * B_scales[column] + bias (int8 A and B; bias may be None)."""
+    s = _stream(stream, A, D)
+    _check(lib().mpk_gemm_int8(_addr(A), lda, _addr(A_scales), _addr(B), ldb, b_layout, _addr(B_scales),
+                               _addr(bias), _addr(D), d_type, ldd, M, N, K, s))
+
+
+def linear_int8_gpu(x, x_type: int, ldx: int, B, ldb: int, b_layout: int, B_scales, bias, D, d_type: int, ldd: int,
+                    M: int, N: int, K: int, stream=None) -> None:
+    """gemm_int8_gpu of x quantized per row on the way."""
+    s = _stream(stream, x, D)
+    _check(lib().mpk_linear_int8(_addr(x), x_type, ldx, _addr(B), ldb, b_layout, _addr(B_scales), _addr(bias),
+                                 _addr(D), d_type, ldd, M, N, K, s))
+
+
+def gemm_grouped_gpu(A, lda: int, B, ldb: int, b_layout: int, ab_type: int, D, d_type: int, ldd: int, offsets,
+                     E: int, M: int, N: int, K: int, stream=None) -> None:
+    """Rows offsets[e]..offsets[e + 1] of D = the same rows of A times B[e] (16-bit types)."""
+    s = _stream(stream, A, D)
+    _check(lib().mpk_gemm_grouped(_addr(A), lda, _addr(B), ldb, b_layout, ab_type, _addr(D), d_type, ldd,
+                                  _addr(offsets), E, M, N, K, s))
+
+
+def gemm_grouped_int8_gpu(A, lda: int, A_scales, B, ldb: int, b_layout: int, B_scales, D, d_type: int, ldd: int,
+                          offsets, E: int, M: int, N: int, K: int, stream=None) -> None:
+    """gemm_grouped_gpu of int8 codes with row scales [M] and column scales [E, N]."""
+    s = _stream(stream, A, D)
+    _check(lib().mpk_gemm_grouped_int8(_addr(A), lda, _addr(A_scales), _addr(B), ldb, b_layout, _addr(B_scales),
+                                       _addr(D), d_type, ldd, _addr(offsets), E, M, N, K, s))
+
+
+def gemm_grouped_mxfp8_gpu(A_data, A_scales, B, ldb: int, D_data, D_scales, offsets, E: int, M: int, N: int, K: int,
+                           stream=None) -> None:
+    """gemm_grouped_gpu with A and D in MXFP8 and B in BF16."""
+    s = _stream(stream, A_data, D_data)
+    _check(lib().mpk_gemm_grouped_mxfp8(_addr(A_data), _addr(A_scales), _addr(B), ldb, _addr(D_data),
+                                        _addr(D_scales), _addr(offsets), E, M, N, K, s))
+
+
+def gemm_grouped_wgrad_gpu(A, lda: int, dD, ldg: int, ab_type: int, dB, d_type: int, ldd: int, offsets, E: int,
+                           M: int, N: int, K: int, stream=None) -> None:
+    """dB[e] [K, N] = A[rows of e]^T * dD[rows of e]; zeros for an empty group."""
+    s = _stream(stream, A, dB)
+    _check(lib().mpk_gemm_grouped_wgrad(_addr(A), lda, _addr(dD), ldg, ab_type, _addr(dB), d_type, ldd,
+                                        _addr(offsets), E, M, N, K, s))
+
+
+# ---------------------------------------------------------------------------
 # Allocating conveniences (torch tensors)
 # ---------------------------------------------------------------------------
 
@@ -410,3 +504,241 @@ def gemm(A_data, A_scales, B, C_data=None, C_scales=None, stream=None):
     Ds = torch.empty((M, nblk(N)), dtype=torch.uint8, device=A_data.device)
     gemm_fp8_tensorcore(A_data, A_scales, B, C_data, C_scales, D, Ds, M, N, K, stream)
     return D, Ds
+
+
+# Allocating forms of the int8 and expert-grouped products.  They take CUDA tensors whose
+# last dimension is contiguous (rows may be strided), check types, shapes and devices,
+# and run on the current stream of the tensors' device.
+
+def _types():
+    import torch
+    return {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+
+
+def _type_code(dtype, what: str, allowed=(TYPE_F32, TYPE_BF16, TYPE_F16)) -> int:
+    code = _types().get(dtype)
+    if code not in allowed:
+        raise ValueError(f"{what}: type {dtype} is not supported")
+    return code
+
+
+def _row_stride(t, what: str) -> int:
+    """Elements between the rows of t [.., rows, columns], matrices back to back."""
+    rows, cols = t.shape[-2], t.shape[-1]
+    st = t.stride()
+    ld = st[-2] if rows > 1 else max(st[-2], cols)
+    if (cols > 1 and st[-1] != 1) or ld < cols:
+        raise ValueError(f"{what}: the last dimension must be contiguous, got strides {tuple(st)}")
+    if t.dim() == 3 and t.shape[0] > 1 and t.numel() > 0 and st[0] != rows * ld:
+        if rows == 1 and st[0] >= cols:
+            return st[0]
+        raise ValueError(f"{what}: the matrices must lie back to back, got strides {tuple(st)}")
+    return ld
+
+
+def _want(t, what: str, dim: int, dtype=None, shape=None, like=None):
+    if not t.is_cuda or t.dim() != dim or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{what}: expected a {dim}-dimensional CUDA tensor"
+                         f"{'' if dtype is None else f' of {dtype}'}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{what} is on {t.device}, not on {like.device}")
+
+
+def _vector(t, what: str, dtype, shape, like):
+    _want(t, what, len(shape), dtype, shape, like)
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+
+
+def _on(t):
+    import torch
+    return torch.cuda.device(t.device)
+
+
+def _result(out, shape, dtype, like):
+    import torch
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _want(out, "out", len(shape), dtype, shape, like)
+    return out
+
+
+def _padded_codes(shape, like):
+    """int8 codes whose rows start on 16-byte boundaries (read in place by the products)."""
+    import torch
+    ld = (shape[-1] + 15) // 16 * 16
+    return torch.empty(tuple(shape[:-1]) + (ld,), dtype=torch.int8, device=like.device)[..., :shape[-1]], ld
+
+
+def quantize_int8(x):
+    """float32, bfloat16 or float16 [M, K] -> (codes int8 [M, K], scales float32 [M]): one
+    scale per row.  The codes' rows are padded to a multiple of 16 bytes."""
+    import torch
+    _want(x, "x", 2)
+    t = _type_code(x.dtype, "x")
+    M, K = x.shape
+    codes, ld = _padded_codes((M, K), x)
+    scales = torch.empty((M,), dtype=torch.float32, device=x.device)
+    with _on(x):
+        int8_quantize_rows_gpu(x, t, _row_stride(x, "x"), codes, ld, scales, M, K)
+    return codes, scales
+
+
+def quantize_int8_cols(w):
+    """float32, bfloat16 or float16 [K, N] or [E, K, N] -> (codes int8 of the same shape,
+    scales float32 [N] or [E, N]): one scale per column.  The codes' rows are padded to a
+    multiple of 16 bytes."""
+    import torch
+    _want(w, "w", 3 if w.dim() == 3 else 2)
+    t = _type_code(w.dtype, "w")
+    E = w.shape[0] if w.dim() == 3 else 1
+    K, N = w.shape[-2:]
+    codes, ld = _padded_codes(w.shape, w)
+    scales = torch.empty(tuple(w.shape[:-2]) + (N,), dtype=torch.float32, device=w.device)
+    with _on(w):
+        int8_quantize_cols_gpu(w, t, _row_stride(w, "w"), codes, ld, scales, E, K, N)
+    return codes, scales
+
+
+def _b_sizes(B, b_layout: int, K: int) -> int:
+    """N of B [.., K, N] (B_KN) or [.., N, K] (B_NK)."""
+    if b_layout not in (B_KN, B_NK):
+        raise ValueError(f"unknown layout of B {b_layout}")
+    k, n = (B.shape[-2], B.shape[-1]) if b_layout == B_KN else (B.shape[-1], B.shape[-2])
+    if k != K:
+        raise ValueError(f"B {tuple(B.shape)} does not have the {K} rows of the product's reduction")
+    return n
+
+
+def gemm_int8(A, A_scales, B, B_scales, bias=None, out_dtype=None, b_layout: int = B_KN, out=None):
+    """D [M, N] = (A*B) * A_scales[row] * B_scales[column] + bias: int8 A [M, K] and B [K, N]
+    (or [N, K] with b_layout=B_NK), float32 scales and bias; D in out_dtype (default bfloat16)."""
+    import torch
+    _want(A, "A", 2, torch.int8)
+    _want(B, "B", 2, torch.int8, like=A)
+    M, K = A.shape
+    N = _b_sizes(B, b_layout, K)
+    _vector(A_scales, "A_scales", torch.float32, (M,), A)
+    _vector(B_scales, "B_scales", torch.float32, (N,), A)
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, (N,), A)
+    dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
+    d = _type_code(dtype, "D")
+    D = _result(out, (M, N), dtype, A)
+    with _on(A):
+        gemm_int8_gpu(A, _row_stride(A, "A"), A_scales, B, _row_stride(B, "B"), b_layout, B_scales, bias, D, d,
+                      _row_stride(D, "D"), M, N, K)
+    return D
+
+
+def linear_int8(x, B, B_scales, bias=None, out_dtype=None, b_layout: int = B_KN, out=None):
+    """gemm_int8 of x [M, K] (float32, bfloat16 or float16) quantized per row on the way; D in
+    out_dtype (default x's type)."""
+    import torch
+    _want(x, "x", 2)
+    _want(B, "B", 2, torch.int8, like=x)
+    t = _type_code(x.dtype, "x")
+    M, K = x.shape
+    N = _b_sizes(B, b_layout, K)
+    _vector(B_scales, "B_scales", torch.float32, (N,), x)
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, (N,), x)
+    dtype = out_dtype or (x.dtype if out is None else out.dtype)
+    d = _type_code(dtype, "D")
+    D = _result(out, (M, N), dtype, x)
+    with _on(x):
+        linear_int8_gpu(x, t, _row_stride(x, "x"), B, _row_stride(B, "B"), b_layout, B_scales, bias, D, d,
+                        _row_stride(D, "D"), M, N, K)
+    return D
+
+
+def gemm_grouped(A, B, offsets, out_dtype=None, b_layout: int = B_KN, out=None):
+    """Rows offsets[e]:offsets[e + 1] of D [M, N] = the same rows of A [M, K] times B[e]; B
+    [E, K, N] (or [E, N, K] with b_layout=B_NK) of A's type (bfloat16 or float16), offsets
+    int32 [E + 1] on the device.  Rows outside every group keep out's values (and are
+    undefined without out).  The gradient of A is gemm_grouped(dD, B, offsets) with the
+    other b_layout, that of B is gemm_grouped_wgrad(A, dD, offsets)."""
+    import torch
+    _want(A, "A", 2)
+    t = _type_code(A.dtype, "A", (TYPE_BF16, TYPE_F16))
+    _want(B, "B", 3, A.dtype, like=A)
+    M, K = A.shape
+    N = _b_sizes(B, b_layout, K)
+    E = B.shape[0]
+    _vector(offsets, "offsets", torch.int32, (E + 1,), A)
+    dtype = out_dtype or (A.dtype if out is None else out.dtype)
+    d = _type_code(dtype, "D")
+    D = _result(out, (M, N), dtype, A)
+    with _on(A):
+        gemm_grouped_gpu(A, _row_stride(A, "A"), B, _row_stride(B, "B"), b_layout, t, D, d, _row_stride(D, "D"),
+                         offsets, E, M, N, K)
+    return D
+
+
+def gemm_grouped_int8(A, A_scales, B, B_scales, offsets, out_dtype=None, b_layout: int = B_KN, out=None):
+    """gemm_grouped of int8 codes: row scales A_scales [M], column scales B_scales [E, N]; D
+    in out_dtype (default bfloat16)."""
+    import torch
+    _want(A, "A", 2, torch.int8)
+    _want(B, "B", 3, torch.int8, like=A)
+    M, K = A.shape
+    N = _b_sizes(B, b_layout, K)
+    E = B.shape[0]
+    _vector(A_scales, "A_scales", torch.float32, (M,), A)
+    _vector(B_scales, "B_scales", torch.float32, (E, N), A)
+    _vector(offsets, "offsets", torch.int32, (E + 1,), A)
+    dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
+    d = _type_code(dtype, "D")
+    D = _result(out, (M, N), dtype, A)
+    with _on(A):
+        gemm_grouped_int8_gpu(A, _row_stride(A, "A"), A_scales, B, _row_stride(B, "B"), b_layout, B_scales, D, d,
+                              _row_stride(D, "D"), offsets, E, M, N, K)
+    return D
+
+
+def gemm_grouped_mxfp8(A_data, A_scales, B, offsets, out=None):
+    """gemm_grouped with A in MXFP8 (codes [M, K], scales [M, ceil(K/32)]) and bfloat16 B
+    [E, K, N]; returns D in MXFP8 along N (codes [M, N], scales [M, ceil(N/32)])."""
+    import torch
+    _want(A_data, "A_data", 2, torch.uint8)
+    _want(B, "B", 3, torch.bfloat16, like=A_data)
+    M, K = A_data.shape
+    N = _b_sizes(B, B_KN, K)
+    E = B.shape[0]
+    _vector(A_data, "A_data", torch.uint8, (M, K), A_data)
+    _vector(A_scales, "A_scales", torch.uint8, (M, nblk(K)), A_data)
+    _vector(offsets, "offsets", torch.int32, (E + 1,), A_data)
+    D, Ds = out if out is not None else (None, None)
+    D = _result(D, (M, N), torch.uint8, A_data)
+    Ds = _result(Ds, (M, nblk(N)), torch.uint8, A_data)
+    if not D.is_contiguous() or not Ds.is_contiguous():
+        raise ValueError("out must be contiguous")
+    with _on(A_data):
+        gemm_grouped_mxfp8_gpu(A_data, A_scales, B, _row_stride(B, "B"), D, Ds, offsets, E, M, N, K)
+    return D, Ds
+
+
+def gemm_grouped_wgrad(A, dD, offsets, out_dtype=None, out=None):
+    """Gradient of gemm_grouped's B [E, K, N]: dB[e] = A[rows of e]^T * dD[rows of e] (zeros
+    for an empty group), in out_dtype (default A's type)."""
+    import torch
+    _want(A, "A", 2)
+    t = _type_code(A.dtype, "A", (TYPE_BF16, TYPE_F16))
+    M, K = A.shape
+    _want(dD, "dD", 2, A.dtype, like=A)
+    N = dD.shape[1]
+    _want(dD, "dD", 2, A.dtype, (M, N), A)
+    _want(offsets, "offsets", 1, torch.int32, like=A)
+    E = offsets.shape[0] - 1
+    if E < 0:
+        raise ValueError("offsets must hold at least one value")
+    _vector(offsets, "offsets", torch.int32, (E + 1,), A)
+    dtype = out_dtype or (A.dtype if out is None else out.dtype)
+    d = _type_code(dtype, "dB")
+    dB = _result(out, (E, K, N), dtype, A)
+    with _on(A):
+        gemm_grouped_wgrad_gpu(A, _row_stride(A, "A"), dD, _row_stride(dD, "dD"), t, dB, d, _row_stride(dB, "dB"),
+                               offsets, E, M, N, K)
+    return dB

@@ -248,6 +248,26 @@ static void forget_workspace_pool()
     g_pools[dev] = nullptr;
 }
 
+// A workspace of `bytes` bytes on `st` for one call, released with cudaFreeAsync on the
+// same stream: from the library's pool, or, while `st` is being captured, from the
+// device's default pool (the graph's own allocation and free nodes).
+static int take_workspace(size_t bytes, cudaStream_t st, void** ws)
+{
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    if (int rc = from_cuda(cudaStreamIsCapturing(st, &cs), "capture state")) return rc;
+    if (cs != cudaStreamCaptureStatusNone) return from_cuda(cudaMallocAsync(ws, bytes, st), "workspace");
+    cudaError_t e = cudaErrorMemoryAllocation;
+    if (cudaMemPool_t pool = workspace_pool(true)) e = cudaMallocFromPoolAsync(ws, bytes, pool, st);
+    if (e == cudaErrorInvalidValue) {
+        // The pool belonged to a context that cudaDeviceReset destroyed.
+        cudaGetLastError();
+        forget_workspace_pool();
+        if (cudaMemPool_t pool = workspace_pool(true)) e = cudaMallocFromPoolAsync(ws, bytes, pool, st);
+    }
+    if (e != cudaSuccess) cudaGetLastError();
+    return from_cuda(e, "workspace");
+}
+
 int mpk_gemm_mxfp8_bf16(const uint8_t* A_data, const uint8_t* A_scales, const void* B_bf16,
                         const uint8_t* C_data, const uint8_t* C_scales, uint8_t* D_data,
                         uint8_t* D_scales, int M, int N, int K, void* stream)
@@ -606,6 +626,308 @@ int mpk_mxfp8_dequantize_host(const uint8_t* data, const uint8_t* scales, float*
         for (int64_t k = 0; k < K; ++k)
             output[r * K + k] = host_e4m3_to_f32(data[r * K + k]) * host_e8m0_to_f32(scales[r * nblk + k / 32]);
     return MPK_SUCCESS;
+}
+
+// ---------------------------------------------------------------------------
+// int8 quantizers, int8 products and products grouped by expert
+// ---------------------------------------------------------------------------
+static bool float_type(int t) { return t == MPK_TYPE_F32 || t == MPK_TYPE_BF16 || t == MPK_TYPE_F16; }
+static int type_bytes(int t) { return t == MPK_TYPE_F32 ? 4 : t == kTypeInt8 ? 1 : 2; }
+
+// rows x cols elements, rows ld apart, `count` of them back to back: ld >= cols, and
+// the byte size within the 2^40 that a tensor map's stride can express.
+static int check_matrix(const char* what, int64_t count, int64_t rows, int64_t cols, int64_t ld, int bytes)
+{
+    if (ld < cols) {
+        set_last_error("%s: row stride %lld is less than its %lld columns", what, (long long)ld, (long long)cols);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    const double total = (double)count * (double)rows * (double)ld * bytes;
+    if ((double)ld * bytes >= 0x1p40 || (double)rows * (double)ld * bytes >= 0x1p40 || total >= 0x1p62) {
+        set_last_error("%s: %lld x %lld rows of %lld elements are too large", what, (long long)count,
+                       (long long)rows, (long long)ld);
+        return MPK_ERR_UNSUPPORTED;
+    }
+    return MPK_SUCCESS;
+}
+
+static int check_aligned(const void* x, int bytes, const float* scales)
+{
+    if (reinterpret_cast<uintptr_t>(x) % bytes || reinterpret_cast<uintptr_t>(scales) % 4) {
+        set_last_error("the quantizers' input and scales must be aligned to their elements");
+        return MPK_ERR_MISALIGNED;
+    }
+    return MPK_SUCCESS;
+}
+
+int mpk_int8_quantize_rows(const void* x, int x_type, int64_t ldx, int8_t* codes, int64_t ld_codes,
+                           float* scales, int M, int K, void* stream)
+{
+    if (M < 0 || K < 0 || !float_type(x_type)) {
+        set_last_error("int8 row quantizer: negative size M=%d K=%d or unknown type %d", M, K, x_type);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (M == 0) return MPK_SUCCESS;
+    if (!scales || (K > 0 && (!x || !codes))) {
+        set_last_error("null device pointer");
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (int rc = check_matrix("x", 1, M, K, ldx, type_bytes(x_type))) return rc;
+    if (int rc = check_matrix("codes", 1, M, K, ld_codes, 1)) return rc;
+    if (int rc = check_aligned(x, type_bytes(x_type), scales)) return rc;
+    if (int rc = check_arch()) return rc;
+    return from_cuda(launch_int8_quantize_rows(x, x_type, ldx, codes, ld_codes, scales, M, K, (cudaStream_t)stream),
+                     "int8 row quantizer launch");
+}
+
+int mpk_int8_quantize_cols(const void* w, int w_type, int64_t ldw, int8_t* codes, int64_t ld_codes,
+                           float* scales, int E, int K, int N, void* stream)
+{
+    if (E < 0 || K < 0 || N < 0 || !float_type(w_type)) {
+        set_last_error("int8 column quantizer: negative size E=%d K=%d N=%d or unknown type %d", E, K, N, w_type);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (E == 0 || N == 0) return MPK_SUCCESS;
+    if (!scales || (K > 0 && (!w || !codes))) {
+        set_last_error("null device pointer");
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (int rc = check_matrix("w", E, K, N, ldw, type_bytes(w_type))) return rc;
+    if (int rc = check_matrix("codes", E, K, N, ld_codes, 1)) return rc;
+    if (int rc = check_aligned(w, type_bytes(w_type), scales)) return rc;
+    if (int rc = check_arch()) return rc;
+    return from_cuda(launch_int8_quantize_cols(w, w_type, ldw, codes, ld_codes, scales, E, K, N,
+                                               (cudaStream_t)stream),
+                     "int8 column quantizer launch");
+}
+
+// Checks shared by the products.  With wgrad, B is dD [M][N] and D is dB [E][K][N].
+static int validate_product(const ProductArgs& a, const int32_t* offsets, bool grouped, int b_layout)
+{
+    if (a.M < 0 || a.N < 0 || a.K < 0 || a.E < 0) {
+        set_last_error("negative size M=%d N=%d K=%d E=%d", a.M, a.N, a.K, a.E);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (b_layout != MPK_B_KN && b_layout != MPK_B_NK) {
+        set_last_error("unknown layout of B %d", b_layout);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (a.ab_type != kTypeInt8 && a.ab_type != MPK_TYPE_BF16 && a.ab_type != MPK_TYPE_F16) {
+        set_last_error("A and B must be BF16 or FP16, got type %d", a.ab_type);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (a.d_type != kTypeMxfp8 && !float_type(a.d_type)) {
+        set_last_error("unknown type of D %d", a.d_type);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (a.E > MPK_MAX_GROUPS) {
+        set_last_error("%d groups, at most %d", a.E, MPK_MAX_GROUPS);
+        return MPK_ERR_UNSUPPORTED;
+    }
+    if (a.ab_type == kTypeInt8 && a.K > 131071) {
+        // 131072 * 128 * 128 = 2^31 is the first sum that 32 bits cannot hold
+        set_last_error("int8 sums are exact up to K = 131071, got K=%d", a.K);
+        return MPK_ERR_UNSUPPORTED;
+    }
+    const int64_t d_rows = a.wgrad ? a.K : a.M, reduction = a.wgrad ? a.M : a.K;
+    if (a.E == 0 || a.N == 0 || d_rows == 0) return MPK_SUCCESS;
+    if (!a.D || (a.d_type == kTypeMxfp8 && !a.D_scales) || (grouped && !offsets) ||
+        (reduction > 0 && (!a.A || !a.B)) || (a.ab_type == kTypeInt8 && (!a.a_scales || !a.b_scales))) {
+        set_last_error("null device pointer");
+        return MPK_ERR_INVALID_VALUE;
+    }
+    const int eb = type_bytes(a.ab_type), db = a.d_type == kTypeMxfp8 ? 1 : type_bytes(a.d_type);
+    if (int rc = check_matrix("A", 1, a.M, a.K, a.lda, eb)) return rc;
+    if (a.wgrad) {
+        if (int rc = check_matrix("dD", 1, a.M, a.N, a.ldb, eb)) return rc;
+    } else if (int rc = b_layout == MPK_B_NK ? check_matrix("B", a.E, a.N, a.K, a.ldb, eb)
+                                             : check_matrix("B", a.E, a.K, a.N, a.ldb, eb)) {
+        return rc;
+    }
+    if (int rc = check_matrix("D", a.wgrad ? a.E : 1, d_rows, a.N, a.ldd, db)) return rc;
+    if (reinterpret_cast<uintptr_t>(a.D) % db || reinterpret_cast<uintptr_t>(a.A) % eb ||
+        reinterpret_cast<uintptr_t>(a.B) % eb) {
+        set_last_error("A, B and D must be aligned to their elements");
+        return MPK_ERR_MISALIGNED;
+    }
+    for (const void* q : {(const void*)a.a_scales, (const void*)a.b_scales, (const void*)a.bias,
+                          (const void*)offsets})
+        if (reinterpret_cast<uintptr_t>(q) % 4) {
+            set_last_error("scales, bias and offsets must be aligned to their elements");
+            return MPK_ERR_MISALIGNED;
+        }
+    return MPK_SUCCESS;
+}
+
+static bool empty_product(const ProductArgs& a)
+{
+    return a.E == 0 || a.N == 0 || (a.wgrad ? a.K : a.M) == 0;
+}
+
+// Runs a validated product; operands that TMA cannot read in place are copied to
+// padded rows in a workspace first.
+static int run_product(ProductArgs a, cudaStream_t st)
+{
+    if (int rc = check_arch()) return rc;
+    const int eb = type_bytes(a.ab_type);
+    const bool none = (a.wgrad ? a.M : a.K) == 0;  // nothing of A and B is read
+    const int64_t per = 16 / eb;
+    const int64_t b_rows = a.wgrad ? a.M : (int64_t)a.E * (a.b_nk ? a.N : a.K);
+    const int64_t b_cols = a.wgrad || !a.b_nk ? a.N : a.K;
+    const bool copy_a = !none && !product_tma_ok(a.A, a.lda, eb);
+    const bool copy_b = !none && !product_tma_ok(a.B, a.ldb, eb);
+    if (!copy_a && !copy_b) return launch_product(a, st);
+    const int64_t lda = (a.K + per - 1) / per * per, ldb = (b_cols + per - 1) / per * per;
+    const size_t a_bytes = copy_a ? ((size_t)a.M * lda * eb + 255) / 256 * 256 : 0;
+    const size_t b_bytes = copy_b ? (size_t)b_rows * ldb * eb : 0;
+    void* ws = nullptr;
+    if (int rc = take_workspace(a_bytes + b_bytes, st, &ws)) return rc;
+    cudaError_t e = cudaSuccess;
+    if (copy_a) {
+        e = cudaMemcpy2DAsync(ws, (size_t)lda * eb, a.A, (size_t)a.lda * eb, (size_t)a.K * eb, (size_t)a.M,
+                              cudaMemcpyDeviceToDevice, st);
+        a.A = ws;
+        a.lda = lda;
+    }
+    if (copy_b && e == cudaSuccess) {
+        void* b = static_cast<uint8_t*>(ws) + a_bytes;
+        e = cudaMemcpy2DAsync(b, (size_t)ldb * eb, a.B, (size_t)a.ldb * eb, (size_t)b_cols * eb, (size_t)b_rows,
+                              cudaMemcpyDeviceToDevice, st);
+        a.B = b;
+        a.ldb = ldb;
+    }
+    a.after_kernel = false;
+    const int rc = e == cudaSuccess ? launch_product(a, st) : from_cuda(e, "operand row-padding copy");
+    const cudaError_t fe = cudaFreeAsync(ws, st);
+    return rc ? rc : from_cuda(fe, "workspace release");
+}
+
+int mpk_gemm_grouped(const void* A, int64_t lda, const void* B, int64_t ldb, int b_layout, int ab_type, void* D,
+                     int d_type, int64_t ldd, const int32_t* offsets, int E, int M, int N, int K, void* stream)
+{
+    ProductArgs a = {};
+    a.A = A, a.lda = lda, a.B = B, a.ldb = ldb, a.b_nk = b_layout == MPK_B_NK;
+    a.ab_type = ab_type == MPK_TYPE_F32 ? -1 : ab_type;
+    a.D = D, a.d_type = d_type, a.ldd = ldd;
+    a.offsets = offsets, a.E = E, a.M = M, a.N = N, a.K = K;
+    if (a.d_type == kTypeMxfp8) a.d_type = -1;
+    if (int rc = validate_product(a, offsets, true, b_layout)) return rc;
+    return empty_product(a) ? MPK_SUCCESS : run_product(a, (cudaStream_t)stream);
+}
+
+int mpk_gemm_grouped_wgrad(const void* A, int64_t lda, const void* dD, int64_t ldg, int ab_type, void* dB,
+                           int d_type, int64_t ldd, const int32_t* offsets, int E, int M, int N, int K,
+                           void* stream)
+{
+    ProductArgs a = {};
+    a.A = A, a.lda = lda, a.B = dD, a.ldb = ldg;
+    a.ab_type = ab_type == MPK_TYPE_F32 || ab_type == kTypeInt8 ? -1 : ab_type;
+    a.D = dB, a.d_type = d_type == kTypeMxfp8 ? -1 : d_type, a.ldd = ldd;
+    a.offsets = offsets, a.E = E, a.M = M, a.N = N, a.K = K;
+    a.wgrad = true;
+    if (int rc = validate_product(a, offsets, true, MPK_B_KN)) return rc;
+    return empty_product(a) ? MPK_SUCCESS : run_product(a, (cudaStream_t)stream);
+}
+
+static ProductArgs int8_args(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb,
+                             int b_layout, const float* B_scales, void* D, int d_type, int64_t ldd, int E, int M,
+                             int N, int K)
+{
+    ProductArgs a = {};
+    a.A = A, a.lda = lda, a.a_scales = A_scales;
+    a.B = B, a.ldb = ldb, a.b_nk = b_layout == MPK_B_NK, a.b_scales = B_scales;
+    a.ab_type = kTypeInt8;
+    a.D = D, a.d_type = d_type == kTypeMxfp8 ? -1 : d_type, a.ldd = ldd;
+    a.E = E, a.M = M, a.N = N, a.K = K;
+    return a;
+}
+
+int mpk_gemm_int8(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb, int b_layout,
+                  const float* B_scales, const float* bias, void* D, int d_type, int64_t ldd, int M, int N, int K,
+                  void* stream)
+{
+    ProductArgs a = int8_args(A, lda, A_scales, B, ldb, b_layout, B_scales, D, d_type, ldd, 1, M, N, K);
+    a.bias = bias;
+    if (int rc = validate_product(a, nullptr, false, b_layout)) return rc;
+    return empty_product(a) ? MPK_SUCCESS : run_product(a, (cudaStream_t)stream);
+}
+
+int mpk_gemm_grouped_int8(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb,
+                          int b_layout, const float* B_scales, void* D, int d_type, int64_t ldd,
+                          const int32_t* offsets, int E, int M, int N, int K, void* stream)
+{
+    ProductArgs a = int8_args(A, lda, A_scales, B, ldb, b_layout, B_scales, D, d_type, ldd, E, M, N, K);
+    a.offsets = offsets;
+    if (int rc = validate_product(a, offsets, true, b_layout)) return rc;
+    return empty_product(a) ? MPK_SUCCESS : run_product(a, (cudaStream_t)stream);
+}
+
+int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int64_t ldb, int b_layout,
+                    const float* B_scales, const float* bias, void* D, int d_type, int64_t ldd, int M, int N, int K,
+                    void* stream)
+{
+    if (M < 0 || K < 0 || !float_type(x_type)) {
+        set_last_error("negative size M=%d K=%d or unknown type of x %d", M, K, x_type);
+        return MPK_ERR_INVALID_VALUE;
+    }
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int64_t lda = ((int64_t)K + 15) / 16 * 16;
+    const size_t scales_at = ((size_t)M * (size_t)lda + 255) / 256 * 256;
+    // Checked with stand-ins for the codes and scales that the workspace will hold.
+    static const float kScale = 0.0f;
+    ProductArgs a = int8_args(reinterpret_cast<const int8_t*>(&kScale), lda, &kScale, B, ldb, b_layout, B_scales, D,
+                              d_type, ldd, 1, M, N, K);
+    a.bias = bias;
+    if (int rc = validate_product(a, nullptr, false, b_layout)) return rc;
+    if (empty_product(a)) return MPK_SUCCESS;
+    if (K > 0 && !x) {
+        set_last_error("null device pointer");
+        return MPK_ERR_INVALID_VALUE;
+    }
+    if (int rc = check_matrix("x", 1, M, K, ldx, type_bytes(x_type))) return rc;
+    if (int rc = check_aligned(x, type_bytes(x_type), nullptr)) return rc;
+    if (int rc = check_arch()) return rc;
+    void* ws = nullptr;
+    if (int rc = take_workspace(scales_at + 4u * (size_t)M, st, &ws)) return rc;
+    int8_t* codes = static_cast<int8_t*>(ws);
+    float* scales = reinterpret_cast<float*>(codes + scales_at);
+    a.A = codes;
+    a.a_scales = scales;
+    a.after_kernel = true;
+    int rc = from_cuda(launch_int8_quantize_rows(x, x_type, ldx, codes, lda, scales, M, K, st),
+                       "int8 row quantizer launch");
+    if (!rc) rc = run_product(a, st);
+    const cudaError_t fe = cudaFreeAsync(ws, st);
+    return rc ? rc : from_cuda(fe, "workspace release");
+}
+
+int mpk_gemm_grouped_mxfp8(const uint8_t* A_data, const uint8_t* A_scales, const void* B_bf16, int64_t ldb,
+                           uint8_t* D_data, uint8_t* D_scales, const int32_t* offsets, int E, int M, int N, int K,
+                           void* stream)
+{
+    const cudaStream_t st = (cudaStream_t)stream;
+    ProductArgs a = {};
+    a.A = A_scales ? A_data : nullptr;
+    a.lda = ((int64_t)K + 7) / 8 * 8;
+    a.B = B_bf16, a.ldb = ldb, a.ab_type = MPK_TYPE_BF16;
+    a.D = D_data, a.D_scales = D_scales, a.d_type = kTypeMxfp8, a.ldd = N;
+    a.offsets = offsets, a.E = E, a.M = M, a.N = N, a.K = K;
+    {
+        ProductArgs checked = a;  // A's own copy in the workspace is aligned whatever A_data is
+        if (a.A) checked.A = &checked;
+        if (int rc = validate_product(checked, offsets, true, MPK_B_KN)) return rc;
+    }
+    if (empty_product(a)) return MPK_SUCCESS;
+    if (K == 0) return run_product(a, st);
+    if (int rc = check_arch()) return rc;
+    void* ws = nullptr;
+    if (int rc = take_workspace((size_t)M * (size_t)a.lda * 2u, st, &ws)) return rc;
+    a.A = ws;
+    a.after_kernel = true;
+    int rc = from_cuda(launch_mxfp8_dequantize_bf16(A_data, A_scales, ws, M, K, a.lda, st), "A pre-pass launch");
+    if (!rc) rc = run_product(a, st);
+    const cudaError_t fe = cudaFreeAsync(ws, st);
+    return rc ? rc : from_cuda(fe, "workspace release");
 }
 
 int mpk_device_status(int* device_status)

@@ -1676,6 +1676,32 @@ int encode_2d(PFN_cuTensorMapEncodeTiled_v12000 enc, CUtensorMap* map, CUtensorM
 
 }  // namespace
 
+int kernel_device_context(int& dev, int** status)
+{
+    if (int rc = get_device(dev)) return rc;
+    return status_ptr(dev, status);
+}
+
+int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int rank, const uint64_t* dims,
+                      const uint64_t* strides_bytes, const uint32_t* box)
+{
+    PFN_cuTensorMapEncodeTiled_v12000 enc;
+    if (int rc = get_encoder(&enc)) return rc;
+    cuuint64_t d[3], st[2];
+    cuuint32_t bx[3];
+    const cuuint32_t estr[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) d[i] = dims[i], bx[i] = box[i];
+    for (int i = 0; i + 1 < rank; ++i) st[i] = strides_bytes[i];
+    const CUresult r = enc(map, dt, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+        return MPK_ERR_DRIVER;
+    }
+    return MPK_SUCCESS;
+}
+
 namespace {
 
 // Shared host setup of both GEMM kernels: device checks, status word, B tensor map

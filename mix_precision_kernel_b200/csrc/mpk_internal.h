@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace mpk {
@@ -89,6 +90,46 @@ int gemm_schedule();
 // Cross-GPU barrier over flag arrays (flags[i]: GPU i's array, at least `world`
 // uint32 slots, peer-accessible); bounded wait, expiry recorded in the status word.
 int launch_peer_barrier(uint32_t* const* flags, int rank, int world, uint32_t epoch, cudaStream_t stream);
+
+// Current device's ordinal and the address of its status word (gemm.cu).
+int kernel_device_context(int& dev, int** status);
+// Tensor map of 128-byte swizzled boxes over a row-major tensor of rank 2 or 3
+// (dims and box innermost first; strides of dims 1.. in bytes).
+int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int rank, const uint64_t* dims,
+                      const uint64_t* strides_bytes, const uint32_t* box);
+
+// int8 quantizers (int8.cu).  `type` is an MPK_TYPE_* value; arguments are validated
+// by the ABI layer.
+cudaError_t launch_int8_quantize_rows(const void* x, int type, int64_t ldx, int8_t* codes, int64_t ld_codes,
+                                      float* scales, int64_t M, int64_t K, cudaStream_t stream);
+cudaError_t launch_int8_quantize_cols(const void* w, int type, int64_t ldw, int8_t* codes, int64_t ld_codes,
+                                      float* scales, int64_t E, int64_t K, int64_t N, cudaStream_t stream);
+
+// Products grouped by expert and int8 products (products.cu).
+struct ProductArgs {
+    const void* A;           // rows product: [M][K], rows lda apart; weight gradient: the same
+    int64_t lda;
+    const void* B;           // rows product: [E][K][N] or [E][N][K], rows ldb apart; weight gradient: dD [M][N]
+    int64_t ldb;
+    int b_nk;                // B is [E][N][K]
+    int ab_type;             // MPK_TYPE_BF16, MPK_TYPE_F16 or kTypeInt8
+    void* D;                 // rows product: [M][N]; weight gradient: [E][K][N]; rows ldd apart
+    int64_t ldd;
+    int d_type;              // MPK_TYPE_* or kTypeMxfp8
+    uint8_t* D_scales;       // kTypeMxfp8 only: [M][ceil(N/32)]
+    const float* a_scales;   // int8 only: [M]
+    const float* b_scales;   // int8 only: [E][N]
+    const float* bias;       // int8 only: [N] or null
+    const int32_t* offsets;  // [E + 1] on the device; null: one group of all rows (E == 1)
+    int E, M, N, K;
+    bool wgrad;
+    bool after_kernel;       // launched right behind a kernel of this library that allows dependents
+};
+constexpr int kTypeInt8 = 16, kTypeMxfp8 = 17;
+constexpr int kMaxGroups = 1024;
+// Operands TMA can read in place: base and row strides multiples of 16 bytes.
+bool product_tma_ok(const void* p, int64_t ld, int elem_bytes);
+int launch_product(const ProductArgs& a, cudaStream_t stream);
 
 // Device-side status word of the GEMM kernels (gemm.cu): read and clear.
 int read_and_clear_device_status(int* value);
