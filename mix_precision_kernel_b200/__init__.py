@@ -90,6 +90,8 @@ def library_path() -> str:
 def lib() -> ctypes.CDLL:
     """Load libmpk.so (built in-tree by ``mix_precision_kernel_b200.build``)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(_LIB_PATH):
@@ -508,15 +510,24 @@ def gemm(A_data, A_scales, B, C_data=None, C_scales=None, stream=None):
 
 # Allocating forms of the int8 and expert-grouped products.  They take CUDA tensors whose
 # last dimension is contiguous (rows may be strided), check types, shapes and devices,
-# and run on the current stream of the tensors' device.
+# and run on the current stream of the tensors' device.  A decoding step makes many such
+# calls of a few microseconds each, so the checks are written out as plain comparisons
+# (`_want` and `_vector` run on the way to an error only).
 
-def _types():
+_torch = None
+_types: dict = {}
+
+
+def _init_torch():
+    global _torch
     import torch
-    return {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+    _types.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16})
+    _torch = torch
+    return torch
 
 
 def _type_code(dtype, what: str, allowed=(TYPE_F32, TYPE_BF16, TYPE_F16)) -> int:
-    code = _types().get(dtype)
+    code = _types.get(dtype)
     if code not in allowed:
         raise ValueError(f"{what}: type {dtype} is not supported")
     return code
@@ -524,12 +535,13 @@ def _type_code(dtype, what: str, allowed=(TYPE_F32, TYPE_BF16, TYPE_F16)) -> int
 
 def _row_stride(t, what: str) -> int:
     """Elements between the rows of t [.., rows, columns], matrices back to back."""
-    rows, cols = t.shape[-2], t.shape[-1]
-    st = t.stride()
-    ld = st[-2] if rows > 1 else max(st[-2], cols)
+    shape, st = t.shape, t.stride()
+    rows, cols, ld = shape[-2], shape[-1], st[-2]
+    if rows <= 1 and ld < cols:
+        ld = cols
     if (cols > 1 and st[-1] != 1) or ld < cols:
         raise ValueError(f"{what}: the last dimension must be contiguous, got strides {tuple(st)}")
-    if t.dim() == 3 and t.shape[0] > 1 and t.numel() > 0 and st[0] != rows * ld:
+    if len(st) == 3 and shape[0] > 1 and st[0] != rows * ld and t.numel() > 0:
         if rows == 1 and st[0] >= cols:
             return st[0]
         raise ValueError(f"{what}: the matrices must lie back to back, got strides {tuple(st)}")
@@ -546,43 +558,64 @@ def _want(t, what: str, dim: int, dtype=None, shape=None, like=None):
         raise ValueError(f"{what} is on {t.device}, not on {like.device}")
 
 
-def _vector(t, what: str, dtype, shape, like):
-    _want(t, what, len(shape), dtype, shape, like)
-    if not t.is_contiguous():
+def _matrix(t, what: str, dim: int, dtype, like=None):
+    """t's shape: a `dim`-dimensional CUDA tensor of dtype (None: any) on like's device."""
+    shape = t.shape
+    if (len(shape) != dim or (dtype is not None and t.dtype is not dtype) or not t.is_cuda
+            or (like is not None and t.get_device() != like.get_device())):
+        _want(t, what, dim, dtype, None, like)
+    return shape
+
+
+def _vector(t, what: str, dtype, shape: tuple, like):
+    if (t.dtype is not dtype or t.shape != shape or t.get_device() != like.get_device() or not t.is_contiguous()):
+        _want(t, what, len(shape), dtype, shape, like)
         raise ValueError(f"{what} must be contiguous")
 
 
-def _on(t):
-    import torch
-    return torch.cuda.device(t.device)
-
-
-def _result(out, shape, dtype, like):
-    import torch
+def _result(out, shape: tuple, dtype, like):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    _want(out, "out", len(shape), dtype, shape, like)
+        return like.new_empty(shape, dtype=dtype)
+    if out.shape != shape or out.dtype is not dtype or out.get_device() != like.get_device():
+        _want(out, "out", len(shape), dtype, shape, like)
     return out
+
+
+def _launch(fn, like, *args):
+    """Call a C entry point on the current stream of like's device."""
+    index = like.get_device()
+    cuda = _torch.cuda
+    if cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status != MPK_SUCCESS:
+        _check(status)
+
+
+def _raw_stream(index: int) -> int:
+    get = getattr(_torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else _torch.cuda.current_stream(index).cuda_stream
 
 
 def _padded_codes(shape, like):
     """int8 codes whose rows start on 16-byte boundaries (read in place by the products)."""
-    import torch
     ld = (shape[-1] + 15) // 16 * 16
-    return torch.empty(tuple(shape[:-1]) + (ld,), dtype=torch.int8, device=like.device)[..., :shape[-1]], ld
+    codes = like.new_empty(tuple(shape[:-1]) + (ld,), dtype=_torch.int8)
+    return (codes if ld == shape[-1] else codes[..., :shape[-1]]), ld
 
 
 def quantize_int8(x):
     """float32, bfloat16 or float16 [M, K] -> (codes int8 [M, K], scales float32 [M]): one
     scale per row.  The codes' rows are padded to a multiple of 16 bytes."""
-    import torch
-    _want(x, "x", 2)
+    torch = _torch or _init_torch()
+    M, K = _matrix(x, "x", 2, None)
     t = _type_code(x.dtype, "x")
-    M, K = x.shape
+    ldx = _row_stride(x, "x")
     codes, ld = _padded_codes((M, K), x)
-    scales = torch.empty((M,), dtype=torch.float32, device=x.device)
-    with _on(x):
-        int8_quantize_rows_gpu(x, t, _row_stride(x, "x"), codes, ld, scales, M, K)
+    scales = x.new_empty((M,), dtype=torch.float32)
+    _launch(lib().mpk_int8_quantize_rows, x, x.data_ptr(), t, ldx, codes.data_ptr(), ld, scales.data_ptr(), M, K)
     return codes, scales
 
 
@@ -590,36 +623,37 @@ def quantize_int8_cols(w):
     """float32, bfloat16 or float16 [K, N] or [E, K, N] -> (codes int8 of the same shape,
     scales float32 [N] or [E, N]): one scale per column.  The codes' rows are padded to a
     multiple of 16 bytes."""
-    import torch
-    _want(w, "w", 3 if w.dim() == 3 else 2)
+    torch = _torch or _init_torch()
+    shape = _matrix(w, "w", 3 if w.dim() == 3 else 2, None)
     t = _type_code(w.dtype, "w")
-    E = w.shape[0] if w.dim() == 3 else 1
-    K, N = w.shape[-2:]
-    codes, ld = _padded_codes(w.shape, w)
-    scales = torch.empty(tuple(w.shape[:-2]) + (N,), dtype=torch.float32, device=w.device)
-    with _on(w):
-        int8_quantize_cols_gpu(w, t, _row_stride(w, "w"), codes, ld, scales, E, K, N)
+    E = shape[0] if len(shape) == 3 else 1
+    K, N = shape[-2:]
+    ldw = _row_stride(w, "w")
+    codes, ld = _padded_codes(shape, w)
+    scales = w.new_empty(tuple(shape[:-2]) + (N,), dtype=torch.float32)
+    _launch(lib().mpk_int8_quantize_cols, w, w.data_ptr(), t, ldw, codes.data_ptr(), ld, scales.data_ptr(), E, K, N)
     return codes, scales
 
 
-def _b_sizes(B, b_layout: int, K: int) -> int:
+def _b_sizes(shape, b_layout: int, K: int) -> int:
     """N of B [.., K, N] (B_KN) or [.., N, K] (B_NK)."""
-    if b_layout not in (B_KN, B_NK):
+    if b_layout == B_KN:
+        k, n = shape[-2], shape[-1]
+    elif b_layout == B_NK:
+        n, k = shape[-2], shape[-1]
+    else:
         raise ValueError(f"unknown layout of B {b_layout}")
-    k, n = (B.shape[-2], B.shape[-1]) if b_layout == B_KN else (B.shape[-1], B.shape[-2])
     if k != K:
-        raise ValueError(f"B {tuple(B.shape)} does not have the {K} rows of the product's reduction")
+        raise ValueError(f"B {tuple(shape)} does not fit a reduction of {K}")
     return n
 
 
 def gemm_int8(A, A_scales, B, B_scales, bias=None, out_dtype=None, b_layout: int = B_KN, out=None):
     """D [M, N] = (A*B) * A_scales[row] * B_scales[column] + bias: int8 A [M, K] and B [K, N]
     (or [N, K] with b_layout=B_NK), float32 scales and bias; D in out_dtype (default bfloat16)."""
-    import torch
-    _want(A, "A", 2, torch.int8)
-    _want(B, "B", 2, torch.int8, like=A)
-    M, K = A.shape
-    N = _b_sizes(B, b_layout, K)
+    torch = _torch or _init_torch()
+    M, K = _matrix(A, "A", 2, torch.int8)
+    N = _b_sizes(_matrix(B, "B", 2, torch.int8, A), b_layout, K)
     _vector(A_scales, "A_scales", torch.float32, (M,), A)
     _vector(B_scales, "B_scales", torch.float32, (N,), A)
     if bias is not None:
@@ -627,30 +661,28 @@ def gemm_int8(A, A_scales, B, B_scales, bias=None, out_dtype=None, b_layout: int
     dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
     d = _type_code(dtype, "D")
     D = _result(out, (M, N), dtype, A)
-    with _on(A):
-        gemm_int8_gpu(A, _row_stride(A, "A"), A_scales, B, _row_stride(B, "B"), b_layout, B_scales, bias, D, d,
-                      _row_stride(D, "D"), M, N, K)
+    _launch(lib().mpk_gemm_int8, A, A.data_ptr(), _row_stride(A, "A"), A_scales.data_ptr(), B.data_ptr(),
+            _row_stride(B, "B"), b_layout, B_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+            D.data_ptr(), d, _row_stride(D, "D"), M, N, K)
     return D
 
 
 def linear_int8(x, B, B_scales, bias=None, out_dtype=None, b_layout: int = B_KN, out=None):
     """gemm_int8 of x [M, K] (float32, bfloat16 or float16) quantized per row on the way; D in
     out_dtype (default x's type)."""
-    import torch
-    _want(x, "x", 2)
-    _want(B, "B", 2, torch.int8, like=x)
+    torch = _torch or _init_torch()
+    M, K = _matrix(x, "x", 2, None)
     t = _type_code(x.dtype, "x")
-    M, K = x.shape
-    N = _b_sizes(B, b_layout, K)
+    N = _b_sizes(_matrix(B, "B", 2, torch.int8, x), b_layout, K)
     _vector(B_scales, "B_scales", torch.float32, (N,), x)
     if bias is not None:
         _vector(bias, "bias", torch.float32, (N,), x)
     dtype = out_dtype or (x.dtype if out is None else out.dtype)
     d = _type_code(dtype, "D")
     D = _result(out, (M, N), dtype, x)
-    with _on(x):
-        linear_int8_gpu(x, t, _row_stride(x, "x"), B, _row_stride(B, "B"), b_layout, B_scales, bias, D, d,
-                        _row_stride(D, "D"), M, N, K)
+    _launch(lib().mpk_linear_int8, x, x.data_ptr(), t, _row_stride(x, "x"), B.data_ptr(), _row_stride(B, "B"),
+            b_layout, B_scales.data_ptr(), None if bias is None else bias.data_ptr(), D.data_ptr(), d,
+            _row_stride(D, "D"), M, N, K)
     return D
 
 
@@ -660,53 +692,49 @@ def gemm_grouped(A, B, offsets, out_dtype=None, b_layout: int = B_KN, out=None):
     int32 [E + 1] on the device.  Rows outside every group keep out's values (and are
     undefined without out).  The gradient of A is gemm_grouped(dD, B, offsets) with the
     other b_layout, that of B is gemm_grouped_wgrad(A, dD, offsets)."""
-    import torch
-    _want(A, "A", 2)
+    torch = _torch or _init_torch()
+    M, K = _matrix(A, "A", 2, None)
     t = _type_code(A.dtype, "A", (TYPE_BF16, TYPE_F16))
-    _want(B, "B", 3, A.dtype, like=A)
-    M, K = A.shape
-    N = _b_sizes(B, b_layout, K)
-    E = B.shape[0]
+    b_shape = _matrix(B, "B", 3, A.dtype, A)
+    N = _b_sizes(b_shape, b_layout, K)
+    E = b_shape[0]
     _vector(offsets, "offsets", torch.int32, (E + 1,), A)
     dtype = out_dtype or (A.dtype if out is None else out.dtype)
     d = _type_code(dtype, "D")
     D = _result(out, (M, N), dtype, A)
-    with _on(A):
-        gemm_grouped_gpu(A, _row_stride(A, "A"), B, _row_stride(B, "B"), b_layout, t, D, d, _row_stride(D, "D"),
-                         offsets, E, M, N, K)
+    _launch(lib().mpk_gemm_grouped, A, A.data_ptr(), _row_stride(A, "A"), B.data_ptr(), _row_stride(B, "B"),
+            b_layout, t, D.data_ptr(), d, _row_stride(D, "D"), offsets.data_ptr(), E, M, N, K)
     return D
 
 
 def gemm_grouped_int8(A, A_scales, B, B_scales, offsets, out_dtype=None, b_layout: int = B_KN, out=None):
     """gemm_grouped of int8 codes: row scales A_scales [M], column scales B_scales [E, N]; D
     in out_dtype (default bfloat16)."""
-    import torch
-    _want(A, "A", 2, torch.int8)
-    _want(B, "B", 3, torch.int8, like=A)
-    M, K = A.shape
-    N = _b_sizes(B, b_layout, K)
-    E = B.shape[0]
+    torch = _torch or _init_torch()
+    M, K = _matrix(A, "A", 2, torch.int8)
+    b_shape = _matrix(B, "B", 3, torch.int8, A)
+    N = _b_sizes(b_shape, b_layout, K)
+    E = b_shape[0]
     _vector(A_scales, "A_scales", torch.float32, (M,), A)
     _vector(B_scales, "B_scales", torch.float32, (E, N), A)
     _vector(offsets, "offsets", torch.int32, (E + 1,), A)
     dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
     d = _type_code(dtype, "D")
     D = _result(out, (M, N), dtype, A)
-    with _on(A):
-        gemm_grouped_int8_gpu(A, _row_stride(A, "A"), A_scales, B, _row_stride(B, "B"), b_layout, B_scales, D, d,
-                              _row_stride(D, "D"), offsets, E, M, N, K)
+    _launch(lib().mpk_gemm_grouped_int8, A, A.data_ptr(), _row_stride(A, "A"), A_scales.data_ptr(), B.data_ptr(),
+            _row_stride(B, "B"), b_layout, B_scales.data_ptr(), D.data_ptr(), d, _row_stride(D, "D"),
+            offsets.data_ptr(), E, M, N, K)
     return D
 
 
 def gemm_grouped_mxfp8(A_data, A_scales, B, offsets, out=None):
     """gemm_grouped with A in MXFP8 (codes [M, K], scales [M, ceil(K/32)]) and bfloat16 B
     [E, K, N]; returns D in MXFP8 along N (codes [M, N], scales [M, ceil(N/32)])."""
-    import torch
-    _want(A_data, "A_data", 2, torch.uint8)
-    _want(B, "B", 3, torch.bfloat16, like=A_data)
-    M, K = A_data.shape
-    N = _b_sizes(B, B_KN, K)
-    E = B.shape[0]
+    torch = _torch or _init_torch()
+    M, K = _matrix(A_data, "A_data", 2, torch.uint8)
+    b_shape = _matrix(B, "B", 3, torch.bfloat16, A_data)
+    N = _b_sizes(b_shape, B_KN, K)
+    E = b_shape[0]
     _vector(A_data, "A_data", torch.uint8, (M, K), A_data)
     _vector(A_scales, "A_scales", torch.uint8, (M, nblk(K)), A_data)
     _vector(offsets, "offsets", torch.int32, (E + 1,), A_data)
@@ -715,30 +743,27 @@ def gemm_grouped_mxfp8(A_data, A_scales, B, offsets, out=None):
     Ds = _result(Ds, (M, nblk(N)), torch.uint8, A_data)
     if not D.is_contiguous() or not Ds.is_contiguous():
         raise ValueError("out must be contiguous")
-    with _on(A_data):
-        gemm_grouped_mxfp8_gpu(A_data, A_scales, B, _row_stride(B, "B"), D, Ds, offsets, E, M, N, K)
+    _launch(lib().mpk_gemm_grouped_mxfp8, A_data, A_data.data_ptr(), A_scales.data_ptr(), B.data_ptr(),
+            _row_stride(B, "B"), D.data_ptr(), Ds.data_ptr(), offsets.data_ptr(), E, M, N, K)
     return D, Ds
 
 
 def gemm_grouped_wgrad(A, dD, offsets, out_dtype=None, out=None):
     """Gradient of gemm_grouped's B [E, K, N]: dB[e] = A[rows of e]^T * dD[rows of e] (zeros
     for an empty group), in out_dtype (default A's type)."""
-    import torch
-    _want(A, "A", 2)
+    torch = _torch or _init_torch()
+    M, K = _matrix(A, "A", 2, None)
     t = _type_code(A.dtype, "A", (TYPE_BF16, TYPE_F16))
-    M, K = A.shape
-    _want(dD, "dD", 2, A.dtype, like=A)
-    N = dD.shape[1]
-    _want(dD, "dD", 2, A.dtype, (M, N), A)
-    _want(offsets, "offsets", 1, torch.int32, like=A)
-    E = offsets.shape[0] - 1
+    rows, N = _matrix(dD, "dD", 2, A.dtype, A)
+    if rows != M:
+        raise ValueError(f"dD has {rows} rows, A has {M}")
+    E = _matrix(offsets, "offsets", 1, torch.int32, A)[0] - 1
     if E < 0:
         raise ValueError("offsets must hold at least one value")
     _vector(offsets, "offsets", torch.int32, (E + 1,), A)
     dtype = out_dtype or (A.dtype if out is None else out.dtype)
     d = _type_code(dtype, "dB")
     dB = _result(out, (E, K, N), dtype, A)
-    with _on(A):
-        gemm_grouped_wgrad_gpu(A, _row_stride(A, "A"), dD, _row_stride(dD, "dD"), t, dB, d, _row_stride(dB, "dB"),
-                               offsets, E, M, N, K)
+    _launch(lib().mpk_gemm_grouped_wgrad, A, A.data_ptr(), _row_stride(A, "A"), dD.data_ptr(), _row_stride(dD, "dD"),
+            t, dB.data_ptr(), d, _row_stride(dB, "dB"), offsets.data_ptr(), E, M, N, K)
     return dB

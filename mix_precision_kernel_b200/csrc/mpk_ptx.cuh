@@ -523,6 +523,16 @@ __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads)
     asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(nthreads) : "memory");
 }
 
+// True in one lane of a converged warp.  Unlike a test of the lane number, the compiler
+// knows that what it guards runs in a single lane, and issues TMA and MMA instructions
+// there without a loop over the warp's lanes.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0u;
+}
+
 // 32-bit store into a CTA of this cluster (shared::cluster address from mapa_shared).
 __device__ __forceinline__ void st_shared_cluster_u32(uint32_t cluster_addr, uint32_t v)
 {

@@ -8,21 +8,30 @@
 //   weight gradient   D[e] = A[rows of e]^T * B[rows of e], a K x N matrix per group
 //                     whose reduction is as long as the group.
 //
+// Orientation.  The columns of D lie on the MMA's M axis (128 per CTA, one tensor-memory
+// lane each) and the rows of D on its N axis (one tensor-memory column each).  N can be
+// any multiple of 16 up to 256 per MMA, so a group of r rows costs a tile about r wide
+// instead of a multiple of 128 or 256: a group of up to 256 rows reads its weights once,
+// and a few tokens cost hardly more than the weights' bytes.  A warp then holds 32
+// neighbouring columns of one row of D and stores them together, whatever D's alignment.
+//
 // The groups' bounds are read from device memory, so that a router's result needs no
 // copy to the host: every CTA scans them into shared memory (row ranges and a running
-// count of tiles) and walks the tiles of all groups with a stride of the grid.
+// count of tiles) and the clusters walk the tiles of all groups with a stride of the grid.
 //
 // Operands stream by TMA into a ring of 128-byte-wide stages (64 16-bit or 128 8-bit
 // elements of the reduction), swizzled as the MMA reads them, in whatever order they
 // are stored: the reduction axis may be the contiguous one (K-major) or the strided
-// one (MN-major) for either operand.  A group's rows start anywhere: a load may begin
-// at any row, and rows of the next group that land in a tile only make accumulator
-// rows that are not stored.  Where the ragged axis is the reduction (weight gradient)
-// the rows behind the group's end are zeroed in shared memory before the last MMAs.
+// one (MN-major).  A group's rows start anywhere: a load may begin at any row, and rows
+// of the next group that land in a tile only make accumulator columns that are not
+// stored.  Where the ragged axis is the reduction (weight gradient) the rows behind the
+// group's end are zeroed in shared memory before the last MMAs.
 //
 // Accumulators live in tensor memory, two of them, so that a tile's epilogue runs
 // under the next tile's MMAs.  FP32 sums for the 16-bit types, 32-bit integer sums
-// (exact: the host refuses a K at which they could overflow) for int8.
+// (exact: the host refuses a K at which they could overflow) for int8.  Where there are
+// fewer tiles than SMs, the CTAs of a cluster share a tile's reduction and join their
+// sums through distributed shared memory in a fixed order (splits).
 //
 // Every mbarrier wait is bounded (mpk::mbar_wait); on expiry the CTA raises an abort
 // flag, records a status code, drains what it has in flight and leaves.
@@ -41,12 +50,23 @@
 namespace mpk {
 namespace product {
 
-constexpr int BM = 128;             // accumulator rows per CTA
+constexpr int kCols = 128;          // columns of D per CTA: tensor-memory lanes
+constexpr int kMaxRows = 256;       // rows of D per tile: tensor-memory columns of an accumulator
 constexpr int kRowBytes = 128;      // reduction bytes per stage
-constexpr int kThreads = 256;       // warps: 0 TMA, 1 MMA, 2 tail rows, 3 idle, 4-7 epilogue
-constexpr int kFirstEpiWarp = 4;
-constexpr int kEpilogueWarps = 4;
+constexpr int kMaxStages = 12;
+constexpr int kEpilogueWarps = 8;
+constexpr int kFirstEpiWarp = 4;    // warps: 0 TMA, 1 MMA, 2 tail rows, 3 idle, 4-11 epilogue
+constexpr int kThreads = 32 * (kFirstEpiWarp + kEpilogueWarps);
+constexpr int P_BYTES = kCols * kRowBytes;  // columns operand per CTA and stage
 constexpr uint64_t kDrainTimeoutNs = 200000000ull;
+
+// Shared memory behind the ring: barriers full, empty, tail [kMaxStages], tfull[2],
+// tempty[2], drain; flags and scan scratch; the table of groups (3 words each).
+constexpr int kNumBars = 3 * kMaxStages + 5;
+constexpr int kMiscOffset = kNumBars * 8;
+constexpr int kScaleOffset = (kMiscOffset + 16 + 4 * (kThreads / 32) + 15) / 16 * 16;  // 32 row scales per warp
+constexpr int kTableOffset = kScaleOffset + 32 * 4 * kEpilogueWarps;
+constexpr int control_bytes(int E) { return kTableOffset + 4 * (3 * E + 1); }
 
 // Wait-site ids reported in the device status word.
 enum { kSiteEmpty = 0x21, kSiteFull = 0x22, kSiteTmemEmpty = 0x23, kSiteTmemFull = 0x24, kSiteTail = 0x25 };
@@ -58,11 +78,15 @@ struct Params {
     int N;               // columns of D
     int num_kb;          // rows product: stages of the reduction
     int num_n_tiles;
-    uint32_t idesc;
+    int splits;          // CTAs (pairs) of a cluster that share a tile's reduction
+    int stages;          // ring stages, each slot_bytes
+    int slot_bytes;
+    int parts_in_ring, parts_offset;  // splits: where their sums meet (offset from the barriers)
+    int tmem_cols, acc_cols;  // tensor memory allocated, and columns from one accumulator to the next
+    uint32_t idesc;      // without N
     uint8_t* D;          // element size from d_type
     int64_t ldd, d_group;  // row and group stride of D, in elements (d_group: weight gradient)
     int d_type;
-    int vec;             // bytes of a store to D (32, 16, or 0: element by element)
     uint8_t* D_scales;
     int nblkN;
     const float* a_scales;
@@ -72,35 +96,20 @@ struct Params {
     uint64_t timeout_ns;
 };
 
-// kInt8: int8 operands, otherwise 16-bit floats.  kAMn / kBMn: the operand's strided
-// axis is the reduction.  kPair: a 2-CTA cluster per tile of 256 rows, otherwise one
-// CTA per tile of 128.  BN: columns per tile.  kMx: D in MXFP8.
-template <bool kInt8_, bool kAMn_, bool kBMn_, bool kPair_, int BN_, int kStages_, bool kMx_>
+// P is the operand of D's columns (weights; dD in a weight gradient), Q that of D's rows
+// (A).  kInt8: int8 operands, otherwise 16-bit floats.  kPMn: P's strided axis is the
+// reduction.  kWgrad: weight gradient, both operands MN-major.  kPair: a 2-CTA pair per
+// tile of 256 columns, otherwise one CTA per tile of 128.  kMx: D in MXFP8.
+template <bool kInt8_, bool kPMn_, bool kWgrad_, bool kPair_, bool kMx_>
 struct Config {
-    static constexpr bool kInt8 = kInt8_, kAMn = kAMn_, kBMn = kBMn_, kPair = kPair_, kMx = kMx_;
-    static constexpr bool kWgrad = kAMn;  // the only product with a ragged reduction
-    static constexpr int BN = BN_, kStages = kStages_;
+    static constexpr bool kInt8 = kInt8_, kPMn = kPMn_, kWgrad = kWgrad_, kPair = kPair_, kMx = kMx_;
+    static_assert(!kWgrad || (kPMn && !kInt8), "a weight gradient's operands are MN-major 16-bit floats");
     static constexpr int kCtas = kPair ? 2 : 1;
-    static constexpr int TM = BM * kCtas;             // tile rows
     static constexpr int BK = kInt8 ? 128 : 64;       // reduction elements per stage
-    static constexpr int kCols = BN / kCtas;          // B columns each CTA loads
     static constexpr int kMnBox = kInt8 ? 128 : 64;   // elements across an MN-major box
-    static constexpr int A_BYTES = BM * kRowBytes;
-    static constexpr int B_BYTES = kCols * kRowBytes;
     static constexpr int kBoxBytes = kRowBytes * BK;  // an MN-major box: BK rows of 128 bytes
+    static constexpr int kRowStep = 16 * kCtas;       // a tile's rows are a multiple
     static constexpr int kFullArrivals = kWgrad && kPair ? 2 : 1;
-    static constexpr uint32_t kTmemCols = 2 * BN;
-    static constexpr int OFF_A = 0;
-    static constexpr int OFF_B = kStages * A_BYTES;
-    static constexpr int OFF_BAR = OFF_B + kStages * B_BYTES;
-    // barriers: full[S], empty[S], tail[S], tfull[2], tempty[2], drain
-    static constexpr int kNumBars = 3 * kStages + 5;
-    static constexpr int OFF_MISC = OFF_BAR + kNumBars * 8;
-    static constexpr int OFF_TABLE = (OFF_MISC + 64 + 15) / 16 * 16;
-    // The table takes 3 words per group behind OFF_TABLE; the launch sizes it.
-    static constexpr int smem_bytes(int E) { return OFF_TABLE + 4 * (3 * E + 1) + 1024; }
-    static_assert(OFF_TABLE + 4 * (3 * kMaxGroups + 1) + 1024 <= 232448, "shared memory of one block");
-    static_assert(kCols % (kBMn ? kMnBox : 8) == 0, "whole boxes of B");
 };
 
 // Row ranges of the groups and the number of tiles before each.
@@ -110,15 +119,18 @@ struct Table {
 
 struct Tile {
     int e;
-    int lo, hi;  // the group's rows
-    int m0, n0;  // tile origin: row within the group (weight gradient: row of D[e]), column
+    int lo, hi;     // the group's rows
+    int r0, rows;   // rows of D: first one within the group (weight gradient: within D[e]) and count
+    int width;      // rows rounded up to what the MMA takes
+    int n0;         // first column
 };
 
-// The tiles of one CTA (pair): t, t + stride, ... in group order, M fastest within
-// panels of kPanelM tiles, so that the tiles in flight share A rows and B columns in L2.
+// The tiles of one cluster: t, t + stride, ... in group order, row tiles fastest within
+// panels of kPanel, so that the tiles in flight share rows and columns in L2.  A group's
+// rows are cut into equal tiles of at most kMaxRows.
 template <class C>
 struct Walk {
-    static constexpr int kPanelM = 8;
+    static constexpr int kPanel = 8;
     int t, stride, e = 0;
     __device__ __forceinline__ Walk(int first, int step) : t(first), stride(step) {}
     __device__ __forceinline__ bool next(const Params& p, const Table& tab, Tile& x)
@@ -130,21 +142,31 @@ struct Walk {
         x.lo = tab.lo[e];
         x.hi = tab.hi[e];
         const int rows = C::kWgrad ? p.out_rows : x.hi - x.lo;
-        const int mt = (rows + C::TM - 1) / C::TM;
-        const int per_panel = kPanelM * p.num_n_tiles;
+        const int mt = (rows + kMaxRows - 1) / kMaxRows;
+        int per = kMaxRows;
+        if constexpr (!C::kWgrad) per = ((rows + mt - 1) / mt + C::kRowStep - 1) / C::kRowStep * C::kRowStep;
+        const int per_panel = kPanel * p.num_n_tiles;
         const int panel = r / per_panel;
         const int q = r - panel * per_panel;
-        const int h = min(kPanelM, mt - panel * kPanelM);
+        const int h = min(kPanel, mt - panel * kPanel);
         const int nt = q / h;
-        x.n0 = nt * C::BN;
-        x.m0 = (panel * kPanelM + q - nt * h) * C::TM;
+        x.n0 = nt * kCols * C::kCtas;
+        x.r0 = (panel * kPanel + q - nt * h) * per;
+        x.rows = min(per, rows - x.r0);
+        x.width = per;
         t += stride;
         return true;
     }
-    // Stages of the reduction of a tile.
-    __device__ __forceinline__ static int stages(const Params& p, const Tile& x)
+    // Stages [k0, k1) of a tile's reduction that split s of p.splits takes.
+    __device__ __forceinline__ static void stages(const Params& p, const Tile& x, int s, int& k0, int& k1)
     {
-        return C::kWgrad ? (x.hi - x.lo + C::BK - 1) / C::BK : p.num_kb;
+        if constexpr (C::kWgrad) {
+            k0 = 0;
+            k1 = (x.hi - x.lo + C::BK - 1) / C::BK;
+        } else {
+            k0 = (int)((int64_t)p.num_kb * s / p.splits);
+            k1 = (int)((int64_t)p.num_kb * (s + 1) / p.splits);
+        }
     }
     // Weight gradient: rows of the last stage that belong to the group, 0 if no row
     // behind them needs zeroing (an MMA takes 16 rows, and MMAs past the end are left out).
@@ -161,7 +183,21 @@ template <class C>
 __device__ void build_table(const Params& p, int* lo, int* hi, int* first, int* scratch)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kPer = kMaxGroups / kThreads;
+    if (p.E == 1) {
+        if (tid == 0) {
+            int a = 0, b = p.M;
+            if (p.offsets != nullptr) {
+                a = min(max(p.offsets[0], 0), p.M);
+                b = min(max(p.offsets[1], a), p.M);
+            }
+            lo[0] = a;
+            hi[0] = b;
+            first[0] = 0;
+            first[1] = ((C::kWgrad ? p.out_rows : b - a) + kMaxRows - 1) / kMaxRows * p.num_n_tiles;
+        }
+        return;
+    }
+    constexpr int kPer = (kMaxGroups + kThreads - 1) / kThreads;
     int count[kPer];
     int sum = 0;
 #pragma unroll
@@ -177,7 +213,7 @@ __device__ void build_table(const Params& p, int* lo, int* hi, int* first, int* 
             lo[e] = a;
             hi[e] = b;
             const int rows = C::kWgrad ? p.out_rows : b - a;
-            count[i] = (rows + C::TM - 1) / C::TM * p.num_n_tiles;
+            count[i] = (rows + kMaxRows - 1) / kMaxRows * p.num_n_tiles;
         }
         sum += count[i];
     }
@@ -200,97 +236,6 @@ __device__ void build_table(const Params& p, int* lo, int* hi, int* first, int* 
             if (e == p.E - 1) first[p.E] = before;
         }
     }
-    __syncthreads();
-}
-
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16)
-{
-    uint32_t r;
-    if (bf16)
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-__device__ __forceinline__ void st_global_32b(void* p, const uint32_t* w)
-{
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
-                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-
-// Store nwords (a multiple of 8) 32-bit words at dst with stores of p.vec bytes.
-template <int kWords>
-__device__ __forceinline__ void store_words(uint8_t* dst, const uint32_t (&w)[kWords], int vec)
-{
-    if (vec == 32) {
-#pragma unroll
-        for (int i = 0; i < kWords; i += 8) st_global_32b(dst + 4 * i, w + i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kWords; i += 4)
-            *reinterpret_cast<uint4*>(dst + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-    }
-}
-
-// 32 columns (the first `valid` of them inside N) of one row of D, rounded once from
-// FP32 to D's type.
-__device__ __forceinline__ void store_row_chunk(const Params& p, int64_t element, int valid, const float (&v)[32])
-{
-    if (p.d_type == MPK_TYPE_F32) {
-        float* dst = reinterpret_cast<float*>(p.D) + element;
-        if (valid == 32 && p.vec) {
-            uint32_t w[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
-            store_words(reinterpret_cast<uint8_t*>(dst), w, p.vec);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i < valid) dst[i] = v[i];
-        }
-    } else {
-        const bool bf16 = p.d_type == MPK_TYPE_BF16;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(p.D) + element;
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], bf16);
-        if (valid == 32 && p.vec) {
-            store_words(reinterpret_cast<uint8_t*>(dst), w, p.vec);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i < valid) dst[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-        }
-    }
-}
-
-// One MX block of a row: the framework's block rule (mx_block_scale), as in the MXFP8
-// GEMM's epilogue.  Columns past N are zeros (their B columns were filled with zeros).
-__device__ __forceinline__ void store_mx_chunk(const Params& p, int64_t row, int col0, int valid, const float (&v)[32])
-{
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));  // NaN ignored
-    float inv;
-    const uint32_t s = mx_block_scale(amax, inv);
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint2 q = quantize8(v + 8 * i, inv);
-        w[2 * i] = q.x;
-        w[2 * i + 1] = q.y;
-    }
-    uint8_t* dst = p.D + row * p.ldd + col0;
-    if (valid == 32 && p.vec) {
-        store_words(dst, w, p.vec);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < valid) dst[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
-    }
-    p.D_scales[row * p.nblkN + col0 / 32] = (uint8_t)s;
 }
 
 template <class C>
@@ -305,140 +250,240 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
     }
 }
 
+// One lane's column of D, and how its sums become elements of D.
 template <class C>
-__device__ __forceinline__ void commit_all(uint32_t bar)
-{
-    if constexpr (C::kPair) umma_commit_pair_mc(bar, 0x3);
-    else umma_commit(bar);
-}
+struct Column {
+    const Params& p;
+    int n;          // column
+    bool ok;        // inside N
+    float sb, bias; // int8: the column's scale and bias
+
+    __device__ __forceinline__ Column(const Params& q, const Tile& x, int col)
+        : p(q), n(col), ok(col < q.N), sb(0.0f), bias(-0.0f)
+    {
+        if (C::kInt8 && ok) {
+            sb = p.b_scales[(int64_t)x.e * p.N + n];
+            if (p.bias != nullptr) bias = p.bias[n];
+        }
+    }
+
+    // Adding -0.0f where there is no bias changes no value.
+    __device__ __forceinline__ float value(uint32_t raw, float sa) const
+    {
+        if constexpr (C::kInt8) return __fadd_rn(__fmul_rn(__fmul_rn((float)(int)raw, sa), sb), bias);
+        return __uint_as_float(raw);
+    }
+
+    // One MX block of row `row`: the 32 lanes of the warp call it together with
+    // neighbouring columns, the first a multiple of 32.  The framework's block rule, as in
+    // the MXFP8 GEMM's epilogue: NaN does not enter the block's amax; columns past N are
+    // zeros or NaN.
+    __device__ __forceinline__ void store_mx(int64_t row, float v) const
+    {
+        const uint32_t mag = __float_as_uint(v) & 0x7FFFFFFFu;
+        const uint32_t amax = __reduce_max_sync(0xFFFFFFFFu, mag > 0x7F800000u ? 0u : mag);
+        float inv;
+        const uint32_t s = mx_block_scale(__uint_as_float(amax), inv);
+        const float q = v * inv;
+        if (ok) p.D[row * p.ldd + n] = (uint8_t)f32x2_to_e4m3x2(q, q);
+        if ((n & 31) == 0 && ok) p.D_scales[row * p.nblkN + n / 32] = (uint8_t)s;
+    }
+
+    template <int kType>
+    __device__ __forceinline__ static void put(uint8_t* at, float v)
+    {
+        if constexpr (kType == MPK_TYPE_F32) *reinterpret_cast<float*>(at) = v;
+        else if constexpr (kType == MPK_TYPE_BF16) *reinterpret_cast<__nv_bfloat16*>(at) = __float2bfloat16_rn(v);
+        else *reinterpret_cast<__half*>(at) = __float2half_rn(v);
+    }
+
+    // `count` rows of this column, `at` the first one's element and `step` bytes between
+    // them; sa: the rows' scales in shared memory (int8).
+    template <int kType>
+    __device__ __forceinline__ void store_rows(const uint32_t (&raw)[32], int count, uint8_t* at, int64_t step,
+                                               const float* sa) const
+    {
+        if (!ok) return;
+        if (count == 32) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if constexpr (C::kInt8) s = *reinterpret_cast<const float4*>(sa + i);
+                put<kType>(at + (i + 0) * step, value(raw[i + 0], s.x));
+                put<kType>(at + (i + 1) * step, value(raw[i + 1], s.y));
+                put<kType>(at + (i + 2) * step, value(raw[i + 2], s.z));
+                put<kType>(at + (i + 3) * step, value(raw[i + 3], s.w));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i < count) put<kType>(at + i * step, value(raw[i], C::kInt8 ? sa[i] : 0.0f));
+        }
+    }
+};
 
 template <class C>
 __global__ void __launch_bounds__(kThreads, 1)
-product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Params p)
+product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
+               const __grid_constant__ CUtensorMap tmap_q16, const Params p)
 {
-    constexpr int S = C::kStages;
+    const int S = p.stages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
-    const uint32_t bar0 = sbase + C::OFF_BAR;
+    uint8_t* control = smem + S * p.slot_bytes;
+    const uint32_t bar0 = smem_u32(control);
     auto full = [&](int s) { return bar0 + 8u * s; };
-    auto empty = [&](int s) { return bar0 + 8u * (S + s); };
-    auto tail = [&](int s) { return bar0 + 8u * (2 * S + s); };
-    auto tfull = [&](int a) { return bar0 + 8u * (3 * S + a); };
-    auto tempty = [&](int a) { return bar0 + 8u * (3 * S + 2 + a); };
-    const uint32_t drain = bar0 + 8u * (3 * S + 4);
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
-    volatile int* never_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
-    int* scratch = reinterpret_cast<int*>(smem + C::OFF_MISC + 16);
-    int* t_lo = reinterpret_cast<int*>(smem + C::OFF_TABLE);
+    auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+    auto tail = [&](int s) { return bar0 + 8u * (2 * kMaxStages + s); };
+    auto tfull = [&](int a) { return bar0 + 8u * (3 * kMaxStages + a); };
+    auto tempty = [&](int a) { return bar0 + 8u * (3 * kMaxStages + 2 + a); };
+    const uint32_t drain = bar0 + 8u * (3 * kMaxStages + 4);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(control + kMiscOffset);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(control + kMiscOffset + 4);
+    volatile int* never_abort = reinterpret_cast<volatile int*>(control + kMiscOffset + 8);
+    int* scratch = reinterpret_cast<int*>(control + kMiscOffset + 16);
+    int* t_lo = reinterpret_cast<int*>(control + kTableOffset);
     int* t_hi = t_lo + p.E;
     int* t_first = t_hi + p.E;
     const Table tab{t_lo, t_hi, t_first};
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t rank = C::kPair ? cluster_ctarank() : 0u;
-    const int unit = C::kPair ? (int)cluster_id_x() : (int)blockIdx.x;
-    const int nunits = C::kPair ? (int)nclusters_x() : (int)gridDim.x;
+    const bool clustered = C::kPair || p.splits > 1;
+    const int ctas = C::kCtas * p.splits;  // of a cluster
+    const int crank = clustered ? (int)cluster_ctarank() : 0;
+    const uint32_t rank = C::kPair ? (uint32_t)(crank & 1) : 0u;  // of the pair
+    const int split = crank / C::kCtas;
+    const uint32_t leader = (uint32_t)(crank - (int)rank);
+    const int unit = (int)blockIdx.x / ctas;
+    const int nunits = (int)gridDim.x / ctas;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) {
-            mbar_init(full(s), C::kFullArrivals);
-            mbar_init(empty(s), 1);
-            mbar_init(tail(s), 1);
+    if (warp == 0) {
+        if (lane < kMaxStages) {
+            mbar_init(full(lane), C::kFullArrivals);
+            mbar_init(empty(lane), 1);
+            mbar_init(tail(lane), 1);
+        } else if (lane < kMaxStages + 2) {
+            mbar_init(tfull(lane - kMaxStages), 1);
+            mbar_init(tempty(lane - kMaxStages), C::kCtas * kEpilogueWarps);
+        } else if (lane == kMaxStages + 2) {
+            mbar_init(drain, 1);
+            *abort_flag = 0;
+            *never_abort = 0;
         }
-        for (int a = 0; a < 2; ++a) {
-            mbar_init(tfull(a), 1);
-            mbar_init(tempty(a), C::kCtas * kEpilogueWarps);
-        }
-        mbar_init(drain, 1);
-        *abort_flag = 0;
-        *never_abort = 0;
         fence_mbar_init();
+    } else if (warp == 3 && p.num_kb > 0) {
+        if (lane == 0) prefetch_tmap(&tmap_p);
+        if (lane == 1) prefetch_tmap(&tmap_q);
+        if (lane == 2 && !C::kWgrad) prefetch_tmap(&tmap_q16);
     }
     if (warp == 1) {
         if constexpr (C::kPair) {
-            tmem_alloc_pair(smem_u32(tmem_holder), C::kTmemCols);
+            tmem_alloc_pair(smem_u32(tmem_holder), p.tmem_cols);
             tmem_relinquish_pair();
         } else {
-            tmem_alloc(smem_u32(tmem_holder), C::kTmemCols);
+            tmem_alloc(smem_u32(tmem_holder), p.tmem_cols);
             tmem_relinquish();
         }
     }
-    // A kernel of this library may still be running in front of this one (codes,
-    // scales or a padded operand): nothing global is touched before it has completed.
-    wait_for_prerequisite_grid();
     build_table<C>(p, t_lo, t_hi, t_first, scratch);
     tc_fence_before();
-    if constexpr (C::kPair) cluster_sync_all();
-    else __syncthreads();
+    __syncthreads();
+    if (clustered) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
     bool producer_aborted = false;
     Walk<C> walk(unit, nunits);
-    Tile x;
+    Tile x = {};
+    auto commit = [&](uint32_t bar) {  // arrive on the barrier in the CTAs of this pair
+        if constexpr (C::kPair) umma_commit_pair_mc(bar, (uint16_t)(0x3u << leader));
+        else umma_commit(bar);
+    };
 
     if (warp == 0) {
         // ------------------------------ TMA producer -------------------------------
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
             uint32_t last_tail = 0, tail_ph = 0;  // per stage: its last use went through tail(s); uses so, mod 2
             bool ok = true;
-            while (ok && walk.next(p, tab, x)) {
-                const int nkb = walk.stages(p, x);
+            auto load_p = [&](int slot, uint32_t bar, int k) {
+                const uint32_t dst = sbase + slot * p.slot_bytes;
+                const int n = x.n0 + kCols * (int)rank;
+                auto load = [&](uint32_t to, int c0, int c1, int c2) {
+                    if constexpr (C::kPair) tma_load_3d_pair(to, &tmap_p, bar, c0, c1, c2);
+                    else tma_load_3d(to, &tmap_p, bar, c0, c1, c2);
+                };
+                if constexpr (C::kPMn) {
+#pragma unroll
+                    for (int j = 0; j < kCols / C::kMnBox; ++j)
+                        load(dst + j * C::kBoxBytes, n + j * C::kMnBox, C::kWgrad ? x.lo + k : k, C::kWgrad ? 0 : x.e);
+                } else {
+                    load(dst, k, n, x.e);
+                }
+            };
+            auto load_q = [&](int slot, uint32_t bar, int k) {
+                const uint32_t dst = sbase + slot * p.slot_bytes + P_BYTES;
+                const int mine = x.width / C::kCtas;  // rows of this CTA
+                const int r = x.r0 + mine * (int)rank;
+                auto load = [&](uint32_t to, const CUtensorMap* map, int c0, int c1) {
+                    if constexpr (C::kPair) tma_load_2d_pair(to, map, bar, c0, c1);
+                    else tma_load_2d(to, map, bar, c0, c1);
+                };
+                if constexpr (C::kWgrad) {
+#pragma unroll
+                    for (int j = 0; j < kMaxRows / C::kCtas / C::kMnBox; ++j)
+                        load(dst + j * C::kBoxBytes, &tmap_q, r + j * C::kMnBox, x.lo + k);
+                } else {
+                    int i = 0;
+                    for (; i + 64 <= mine; i += 64) load(dst + i * kRowBytes, &tmap_q, k, x.lo + r + i);
+                    for (; i < mine; i += 16) load(dst + i * kRowBytes, &tmap_q16, k, x.lo + r + i);
+                }
+            };
+            // The kernel in front of this one (if it allowed this one to start early) makes
+            // Q, never P: the first stages' P loads run under it.
+            const bool have = walk.next(p, tab, x);
+            int k0 = 0, k1 = 0, early = 0;
+            if (have) walk.stages(p, x, split, k0, k1);
+            if (!C::kWgrad && have) {
+                early = min(S, k1 - k0);
+                for (int i = 0; i < early; ++i) {
+                    if (rank == 0)
+                        mbar_arrive_expect_tx(full(i), C::kCtas * (P_BYTES + x.width / C::kCtas * kRowBytes));
+                    load_p(i, C::kPair ? mapa_shared(full(i), leader) : full(i), (k0 + i) * C::BK);
+                }
+            }
+            wait_for_prerequisite_grid();
+            for (bool more = have; ok && more; more = walk.next(p, tab, x)) {
+                walk.stages(p, x, split, k0, k1);
                 const int tail_rows = walk.tail_rows(x);
-                const int m = x.m0 + BM * (int)rank;
-                const int n = x.n0 + C::kCols * (int)rank;
-                for (int kb = 0; kb < nkb; ++kb) {
+                const uint32_t bytes = P_BYTES + x.width / C::kCtas * kRowBytes;
+                for (int kb = k0; kb < k1; ++kb) {
                     if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, p.status, kSiteEmpty, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
                     uint32_t bar;
                     last_tail &= ~(1u << s);
-                    if (C::kWgrad && tail_rows > 0 && kb == nkb - 1) {
+                    if (C::kWgrad && tail_rows > 0 && kb == k1 - 1) {
                         // This CTA's tail warp takes the stage first.
                         bar = tail(s);
                         last_tail |= 1u << s;
                         tail_ph ^= 1u << s;
-                        mbar_arrive_expect_tx(bar, C::A_BYTES + C::B_BYTES);
-                        if constexpr (C::kPair) bar = mapa_shared(bar, rank);
+                        mbar_arrive_expect_tx(bar, bytes);
+                        if constexpr (C::kPair) bar = mapa_shared(bar, leader + rank);
                     } else {
-                        if (rank == 0) {
-                            mbar_arrive_expect_tx(full(s), C::kCtas * (C::A_BYTES + C::B_BYTES));
+                        if (rank == 0 && early == 0) {
+                            mbar_arrive_expect_tx(full(s), C::kCtas * bytes);
                             if (C::kFullArrivals == 2) mbar_arrive(full(s));
                         }
                         bar = full(s);
-                        if constexpr (C::kPair) bar = mapa_shared(bar, 0);
+                        if constexpr (C::kPair) bar = mapa_shared(bar, leader);
                     }
-                    const uint32_t a = sbase + C::OFF_A + s * C::A_BYTES;
-                    const uint32_t b = sbase + C::OFF_B + s * C::B_BYTES;
-                    auto load_a = [&](uint32_t dst, int c0, int c1) {
-                        if constexpr (C::kPair) tma_load_2d_pair(dst, &tmap_a, bar, c0, c1);
-                        else tma_load_2d(dst, &tmap_a, bar, c0, c1);
-                    };
-                    auto load_b = [&](uint32_t dst, int c0, int c1, int c2) {
-                        if constexpr (C::kPair) tma_load_3d_pair(dst, &tmap_b, bar, c0, c1, c2);
-                        else tma_load_3d(dst, &tmap_b, bar, c0, c1, c2);
-                    };
-                    const int k0 = kb * C::BK;
-                    if constexpr (C::kAMn) {
-#pragma unroll
-                        for (int j = 0; j < BM / C::kMnBox; ++j)
-                            load_a(a + j * C::kBoxBytes, m + j * C::kMnBox, x.lo + k0);
-                    } else {
-                        load_a(a, k0, x.lo + m);
-                    }
-                    if constexpr (C::kBMn) {
-#pragma unroll
-                        for (int j = 0; j < C::kCols / C::kMnBox; ++j)
-                            load_b(b + j * C::kBoxBytes, n + j * C::kMnBox, C::kWgrad ? x.lo + k0 : k0,
-                                   C::kWgrad ? 0 : x.e);
-                    } else {
-                        load_b(b, k0, n, x.e);
-                    }
+                    if (early > 0) --early;
+                    else load_p(s, bar, kb * C::BK);
+                    load_q(s, bar, kb * C::BK);
                     ++issued;
                     if (++s == S) { s = 0; ph ^= 1u; }
                 }
@@ -460,12 +505,13 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         }
     } else if (warp == 1) {
         // ------------------------------- MMA issuer --------------------------------
-        if (rank == 0 && lane == 0) {
+        if (rank == 0 && elect_one()) {
             int s = 0, it = 0;
             uint32_t ph = 0;
             bool ok = true;
             for (; ok && walk.next(p, tab, x); ++it) {
-                const int nkb = walk.stages(p, x);
+                int k0, k1;
+                walk.stages(p, x, split, k0, k1);
                 const int acc = it & 1;
                 if (!mbar_wait(tempty(acc), ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.status, kSiteTmemEmpty,
                                p.timeout_ns)) {
@@ -473,54 +519,56 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(acc * C::BN);
+                const uint32_t d = tmem_base + (uint32_t)(acc * p.acc_cols);
+                const uint32_t idesc = p.idesc | ((uint32_t)(x.width >> 3) << 17);
                 const int rem = (x.hi - x.lo) % C::BK;
-                for (int kb = 0; kb < nkb; ++kb) {
+                for (int kb = k0; kb < k1; ++kb) {
                     if (!mbar_wait(full(s), ph, abort_flag, p.status, kSiteFull, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
                     int steps = 4;
-                    if (C::kWgrad && kb == nkb - 1 && rem != 0) {
+                    if (C::kWgrad && kb == k1 - 1 && rem != 0) {
                         steps = (rem + 15) / 16;
                         fence_acq_rel_cluster();  // the tail warps' zeros, of both CTAs
                     }
                     tc_fence_after();
-                    const uint32_t a = sbase + C::OFF_A + s * C::A_BYTES;
-                    const uint32_t b = sbase + C::OFF_B + s * C::B_BYTES;
+                    const uint32_t a = sbase + s * p.slot_bytes;
+                    const uint32_t b = a + P_BYTES;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         if (C::kWgrad && k >= steps) break;
                         // A step is 32 bytes along a K-major row, or BK / 4 rows of an MN-major box.
                         constexpr uint32_t kMnStep = C::BK / 4 * kRowBytes;
-                        const uint64_t ad = C::kAMn ? umma_smem_desc_sw128(a + k * kMnStep, C::kBoxBytes, 1024)
+                        const uint64_t ad = C::kPMn ? umma_smem_desc_sw128(a + k * kMnStep, C::kBoxBytes, 1024)
                                                     : umma_smem_desc_sw128(a + k * 32, 16, 1024);
-                        const uint64_t bd = C::kBMn ? umma_smem_desc_sw128(b + k * kMnStep, C::kBoxBytes, 1024)
-                                                    : umma_smem_desc_sw128(b + k * 32, 16, 1024);
-                        mma<C>(d, ad, bd, p.idesc, (kb != 0 || k != 0) ? 1u : 0u);
+                        const uint64_t bd = C::kWgrad ? umma_smem_desc_sw128(b + k * kMnStep, C::kBoxBytes, 1024)
+                                                      : umma_smem_desc_sw128(b + k * 32, 16, 1024);
+                        mma<C>(d, ad, bd, idesc, (kb != k0 || k != 0) ? 1u : 0u);
                     }
-                    commit_all<C>(empty(s));
+                    commit(empty(s));
                     if (++s == S) { s = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
-                commit_all<C>(tfull(acc));
+                commit(tfull(acc));
             }
             if constexpr (C::kPair) umma_commit_pair(drain);
             else umma_commit(drain);
             mbar_wait(drain, 0, never_abort, nullptr, 0, kDrainTimeoutNs);
         }
     } else if (C::kWgrad && warp == 2) {
-        // ------- tail rows: zeros behind the group's end, in A and in B -------
-        // A zero in A alone would leave NaN where the next group's B holds NaN.
+        // ------- tail rows: zeros behind the group's end, in P and in Q -------
+        // A zero in one operand alone would leave NaN where the next group's other holds NaN.
         int s = 0;
         uint32_t phases = 0;  // parity of each stage's tail barrier
-        const uint32_t full0 = C::kPair ? mapa_shared(full(0), 0) : full(0);
+        const uint32_t full0 = C::kPair ? mapa_shared(full(0), leader) : full(0);
         bool ok = true;
         while (ok && walk.next(p, tab, x)) {
-            const int nkb = walk.stages(p, x);
+            int k0, k1;
+            walk.stages(p, x, split, k0, k1);
             const int rows = walk.tail_rows(x);
-            if (nkb == 0) continue;
-            const int last = (s + nkb - 1) % S;
+            if (k1 == k0) continue;
+            const int last = (s + k1 - k0 - 1) % S;
             s = (last + 1) % S;
             if (rows == 0) continue;
             ok = mbar_wait(tail(last), (phases >> last) & 1u, abort_flag, p.status, kSiteTail, p.timeout_ns);
@@ -529,11 +577,10 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             phases ^= 1u << last;
             const int end = (rows + 15) / 16 * 16;
             // 128-byte rows of each box: the swizzle permutes within a row, so whole rows are plain.
-            constexpr int kABoxes = BM / C::kMnBox, kBBoxes = C::kCols / C::kMnBox;
+            constexpr int kBoxes = (kCols + kMaxRows / C::kCtas) / C::kMnBox;
             const int chunks = (end - rows) * 8;
-            for (int j = 0; j < kABoxes + kBBoxes; ++j) {
-                uint8_t* box = j < kABoxes ? smem + C::OFF_A + last * C::A_BYTES + j * C::kBoxBytes
-                                           : smem + C::OFF_B + last * C::B_BYTES + (j - kABoxes) * C::kBoxBytes;
+            for (int j = 0; j < kBoxes; ++j) {
+                uint8_t* box = smem + last * p.slot_bytes + j * C::kBoxBytes;
                 for (int i = lane; i < chunks; i += 32)
                     reinterpret_cast<uint4*>(box + rows * kRowBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
             }
@@ -546,54 +593,66 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         }
     } else if (warp >= kFirstEpiWarp) {
         // -------------------------------- epilogue ---------------------------------
+        // Two warps per quarter of the columns take turns at chunks of 32 rows.
         const int quad = warp & 3;
-        const int r = quad * 32 + lane;  // accumulator row
-        const uint32_t tempty0 = C::kPair ? mapa_shared(tempty(0), 0) : tempty(0);
-        for (int it = 0; walk.next(p, tab, x); ++it) {
+        const int turn = (warp - kFirstEpiWarp) / 4;
+        const uint32_t tempty0 = C::kPair ? mapa_shared(tempty(0), leader) : tempty(0);
+        float* row_scales = reinterpret_cast<float*>(control + kScaleOffset) + (warp - kFirstEpiWarp) * 32;
+        wait_for_prerequisite_grid();  // a_scales may come from the kernel in front
+        // A cluster of splits has one tile, joined below.
+        for (int it = 0; p.splits == 1 && walk.next(p, tab, x); ++it) {
             const int acc = it & 1;
-            const int rows = C::kWgrad ? p.out_rows : x.hi - x.lo;
-            const int row = x.m0 + BM * (int)rank + r;  // within the group
-            const bool row_ok = row < rows;
-            const bool warp_ok = x.m0 + BM * (int)rank + quad * 32 < rows;
-            const int64_t grow = C::kWgrad ? (int64_t)row : (int64_t)x.lo + row;
-            const int64_t base = (C::kWgrad ? x.e * p.d_group : 0) + grow * p.ldd;
-            const bool any = walk.stages(p, x) > 0;  // otherwise nothing was accumulated: zeros
-            float sa = 0.0f;
-            if (C::kInt8 && row_ok) sa = p.a_scales[grow];  // may be written by the kernel in front: no read-only load
+            const Column<C> col(p, x, x.n0 + kCols * (int)rank + quad * 32 + lane);
+            const bool warp_ok = col.n - lane < p.N;
+            int k0, k1;
+            walk.stages(p, x, split, k0, k1);
+            const bool any = k1 > k0;  // otherwise nothing was accumulated: zeros
+            const int64_t row0 = C::kWgrad ? (int64_t)x.r0 : (int64_t)x.lo + x.r0;
+            const int64_t base0 = (C::kWgrad ? x.e * p.d_group : 0) + row0 * p.ldd;
+            float sa[kMaxRows / 64];  // scale of this lane's row of each chunk, under the MMAs
+            if constexpr (C::kInt8) {
+#pragma unroll
+                for (int j = 0; j < kMaxRows / 64; ++j) {
+                    const int r = 64 * j + 32 * turn + lane;
+                    sa[j] = r < x.rows ? p.a_scales[row0 + r] : 0.0f;
+                }
+            }
             if (!mbar_wait(tfull(acc), (uint32_t)(it >> 1) & 1u, abort_flag, p.status, kSiteTmemFull, p.timeout_ns))
                 break;
             tc_fence_after();
-            const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * C::BN);
+            const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * p.acc_cols);
             if (warp_ok) {
+                int j = 0;
 #pragma unroll 1
-                for (int c = 0; c < C::BN / 32; ++c) {
-                    const int col0 = x.n0 + 32 * c;
-                    if (col0 >= p.N) break;
-                    const int valid = min(32, p.N - col0);
+                for (int c = 32 * turn; c < x.rows; c += 64, ++j) {
                     uint32_t raw[32];
                     if (any) {
-                        tmem_ld_32x32b_x32(trow + 32u * c, raw);
+                        tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
                         tmem_ld_wait();
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) raw[i] = 0u;
                     }
-                    float v[32];
-                    if constexpr (C::kInt8) {
-                        const float* sb = p.b_scales + (int64_t)x.e * p.N + col0;
+                    const int count = min(32, x.rows - c);
+                    if constexpr (C::kMx) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float b = i < valid ? __ldg(sb + i) : 0.0f;
-                            v[i] = __fmul_rn(__fmul_rn((float)(int)raw[i], sa), b);
-                            if (p.bias != nullptr && i < valid) v[i] = __fadd_rn(v[i], __ldg(p.bias + col0 + i));
-                        }
+                        for (int i = 0; i < 32; ++i)
+                            if (i < count) col.store_mx(row0 + c + i, __uint_as_float(raw[i]));  // warp-uniform
                     } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-                    }
-                    if (row_ok) {
-                        if constexpr (C::kMx) store_mx_chunk(p, grow, col0, valid, v);
-                        else store_row_chunk(p, base + col0, valid, v);
+                        if constexpr (C::kInt8) {
+                            __syncwarp();
+                            row_scales[lane] = j == 0 ? sa[0] : j == 1 ? sa[1] : j == 2 ? sa[2] : sa[3];
+                            __syncwarp();
+                        }
+                        const int eb = p.d_type == MPK_TYPE_F32 ? 4 : 2;
+                        uint8_t* at = p.D + (base0 + c * p.ldd + col.n) * eb;
+                        const int64_t step = p.ldd * eb;
+                        if (p.d_type == MPK_TYPE_BF16)
+                            col.template store_rows<MPK_TYPE_BF16>(raw, count, at, step, row_scales);
+                        else if (p.d_type == MPK_TYPE_F16)
+                            col.template store_rows<MPK_TYPE_F16>(raw, count, at, step, row_scales);
+                        else
+                            col.template store_rows<MPK_TYPE_F32>(raw, count, at, step, row_scales);
                     }
                 }
             }
@@ -605,6 +664,73 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             }
         }
     }
+    __syncwarp();
+
+    if (!C::kWgrad && p.splits > 1 && unit < tab.first[p.E]) {
+        // Join the splits' sums in their order.  Row i of the tile is finished by split
+        // i % splits: every CTA hands its part of the row to that split's CTA of the same
+        // columns, as row (i / splits) of its slice `split` there.
+        Walk<C> again(unit, nunits);
+        again.next(p, tab, x);
+        const int quad = warp & 3;
+        const int turn = (warp - kFirstEpiWarp) / 4;
+        const int share = (x.rows + p.splits - 1) / p.splits;  // rows of a slice
+        const Column<C> col(p, x, x.n0 + kCols * (int)rank + quad * 32 + lane);
+        const bool busy = warp >= kFirstEpiWarp && col.n - lane < p.N;
+        // Slices lie in the ring's place if there is no room behind it: then every CTA's
+        // MMAs must be done before the first row arrives.
+        uint8_t* parts = p.parts_in_ring ? smem : control + p.parts_offset;
+        bool ok = true;
+        if (warp >= kFirstEpiWarp) {
+            ok = mbar_wait(tfull(0), 0, abort_flag, p.status, kSiteTmemFull, p.timeout_ns);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            tc_fence_after();
+        }
+        if (p.parts_in_ring) cluster_sync_all();
+        if (busy && ok) {
+            const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16);
+            const uint32_t mine = smem_u32(parts) + 4u * (uint32_t)(split * share * kCols + quad * 32 + lane);
+#pragma unroll 1
+            for (int c = 32 * turn; c < x.rows; c += 64) {
+                uint32_t raw[32];
+                tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
+                tmem_ld_wait();
+                int to = c % p.splits, row = c / p.splits;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if (c + i < x.rows)
+                        st_shared_cluster_u32(mapa_shared(mine + 4u * (uint32_t)(row * kCols),
+                                                          (uint32_t)(to * C::kCtas) + rank), raw[i]);
+                    if (++to == p.splits) to = 0, ++row;
+                }
+            }
+        }
+        cluster_sync_all();
+        if (busy && *abort_flag == 0) {
+            const uint32_t* part = reinterpret_cast<const uint32_t*>(parts) + quad * 32 + lane;
+#pragma unroll 2
+            for (int j = turn; split + j * p.splits < x.rows; j += 2) {
+                uint32_t v[8], sum = part[j * kCols];
+#pragma unroll
+                for (int q = 1; q < 8; ++q) v[q] = q < p.splits ? part[(q * share + j) * kCols] : 0u;
+#pragma unroll
+                for (int q = 1; q < 8; ++q)
+                    if (q < p.splits)
+                        sum = C::kInt8 ? sum + v[q] : __float_as_uint(__uint_as_float(sum) + __uint_as_float(v[q]));
+                const int64_t row = (int64_t)x.lo + x.r0 + split + j * p.splits;
+                const float d = col.value(sum, C::kInt8 ? p.a_scales[row] : 0.0f);
+                if constexpr (C::kMx) {
+                    col.store_mx(row, d);
+                } else if (col.ok) {
+                    uint8_t* at = p.D + (row * p.ldd + col.n) * (p.d_type == MPK_TYPE_F32 ? 4 : 2);
+                    if (p.d_type == MPK_TYPE_BF16) col.template put<MPK_TYPE_BF16>(at, d);
+                    else if (p.d_type == MPK_TYPE_F16) col.template put<MPK_TYPE_F16>(at, d);
+                    else col.template put<MPK_TYPE_F32>(at, d);
+                }
+            }
+        }
+        __syncwarp();
+    }
 
     if (producer_aborted) {
         // A copy of the other CTA may still be landing after rank 0 stopped expecting it.
@@ -614,12 +740,12 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     __syncwarp();
     tc_fence_before();
-    if constexpr (C::kPair) cluster_sync_all();
+    if (clustered) cluster_sync_all();
     else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        if constexpr (C::kPair) tmem_dealloc_pair(tmem_base, C::kTmemCols);
-        else tmem_dealloc(tmem_base, C::kTmemCols);
+        if constexpr (C::kPair) tmem_dealloc_pair(tmem_base, p.tmem_cols);
+        else tmem_dealloc(tmem_base, p.tmem_cols);
     }
 }
 
@@ -631,54 +757,87 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 namespace {
 
 std::mutex g_attr_mu;
+constexpr int kSmemMax = 232448;  // of one block
+
+int pow2_at_least(int x)
+{
+    int p = 32;
+    while (p < x) p *= 2;
+    return p;
+}
 
 template <class C>
-int launch_config(const ProductArgs& a, product::Params& p, int64_t max_tiles, cudaStream_t stream, int dev)
+int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream, int dev)
 {
     using namespace product;
     static bool attr_set[64] = {};
     const int eb = C::kInt8 ? 1 : 2;
-    CUtensorMap ta{}, tb{};
+    CUtensorMap tp{}, tq{}, tq16{};
     const CUtensorMapDataType dt = C::kInt8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : a.ab_type == MPK_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const int reduction = C::kWgrad ? a.M : a.K;
     if (reduction > 0) {  // otherwise no load is issued
-        const uint64_t adims[2] = {(uint64_t)a.K, (uint64_t)a.M};
-        const uint64_t astr[1] = {(uint64_t)a.lda * eb};
-        const uint32_t abox[2] = {(uint32_t)(C::kAMn ? C::kMnBox : C::BK), (uint32_t)(C::kAMn ? C::BK : BM)};
-        if (int rc = encode_tensor_map(&ta, dt, a.A, 2, adims, astr, abox)) return rc;
-        const int b_inner = C::kBMn ? a.N : a.K;
-        const int b_rows = C::kWgrad ? a.M : (C::kBMn ? a.K : a.N);
-        const uint64_t bdims[3] = {(uint64_t)b_inner, (uint64_t)b_rows, (uint64_t)(C::kWgrad ? 1 : a.E)};
-        const uint64_t bstr[2] = {(uint64_t)a.ldb * eb, (uint64_t)a.ldb * eb * (uint64_t)b_rows};
-        const uint32_t bbox[3] = {(uint32_t)(C::kBMn ? C::kMnBox : C::BK), (uint32_t)(C::kBMn ? C::BK : C::kCols), 1u};
-        if (int rc = encode_tensor_map(&tb, dt, a.B, 3, bdims, bstr, bbox)) return rc;
+        const uint64_t qdims[2] = {(uint64_t)a.K, (uint64_t)a.M};
+        const uint64_t qstr[1] = {(uint64_t)a.lda * eb};
+        const uint32_t qbox[2] = {(uint32_t)(C::kWgrad ? C::kMnBox : C::BK), 64u};
+        if (int rc = encode_tensor_map(&tq, dt, a.A, 2, qdims, qstr, qbox)) return rc;
+        if (!C::kWgrad) {
+            const uint32_t qbox16[2] = {(uint32_t)C::BK, 16u};
+            if (int rc = encode_tensor_map(&tq16, dt, a.A, 2, qdims, qstr, qbox16)) return rc;
+        }
+        const int p_inner = C::kPMn ? a.N : a.K;
+        const int p_rows = C::kWgrad ? a.M : (C::kPMn ? a.K : a.N);
+        const uint64_t pdims[3] = {(uint64_t)p_inner, (uint64_t)p_rows, (uint64_t)(C::kWgrad ? 1 : a.E)};
+        const uint64_t pstr[2] = {(uint64_t)a.ldb * eb, (uint64_t)a.ldb * eb * (uint64_t)p_rows};
+        const uint32_t pbox[3] = {(uint32_t)(C::kPMn ? C::kMnBox : C::BK), (uint32_t)(C::kPMn ? C::BK : kCols), 1u};
+        if (int rc = encode_tensor_map(&tp, dt, a.B, 3, pdims, pstr, pbox)) return rc;
     }
     p.num_kb = (a.K + C::BK - 1) / C::BK;
-    p.num_n_tiles = (a.N + C::BN - 1) / C::BN;
+    p.num_n_tiles = (a.N + kCols * C::kCtas - 1) / (kCols * C::kCtas);
     if (C::kInt8)
-        p.idesc = (2u << 4) | (1u << 7) | (1u << 10);  // S32 sums, signed 8-bit A and B
+        p.idesc = (2u << 4) | (1u << 7) | (1u << 10);  // S32 sums, signed 8-bit operands
     else
         p.idesc = (1u << 4) | (a.ab_type == MPK_TYPE_BF16 ? (1u << 7) | (1u << 10) : 0u);  // FP32 sums
-    p.idesc |= ((C::kAMn ? 1u : 0u) << 15) | ((C::kBMn ? 1u : 0u) << 16) | ((uint32_t)(C::BN >> 3) << 17) |
-               ((uint32_t)(C::TM >> 4) << 24);
+    p.idesc |= ((C::kPMn ? 1u : 0u) << 15) | ((C::kWgrad ? 1u : 0u) << 16) |
+               ((uint32_t)(kCols * C::kCtas >> 4) << 24);
 
-    // The walk counts tiles in 32 bits.
-    const int64_t m_tiles = C::kWgrad ? (int64_t)a.E * ((a.K + C::TM - 1) / C::TM)
-                                      : (int64_t)a.M / C::TM + std::min(a.E, a.M);
-    const int64_t tiles = m_tiles * p.num_n_tiles;
-    if (tiles > INT32_MAX / 2) {
-        set_last_error("product of more than 2^30 tiles (M=%d N=%d K=%d, %d groups)", a.M, a.N, a.K, a.E);
+    // At most this many tiles (a group of r rows has ceil(r / kMaxRows) row tiles); the
+    // walk counts them in 32 bits.
+    const int64_t row_tiles = C::kWgrad ? (int64_t)a.E * ((a.K + kMaxRows - 1) / kMaxRows)
+                                        : (int64_t)a.M / kMaxRows + std::min(a.E, a.M);
+    const int64_t tiles = row_tiles * p.num_n_tiles;
+    if (tiles > INT32_MAX / 16) {
+        set_last_error("product of more than 2^27 tiles (M=%d N=%d K=%d, %d groups)", a.M, a.N, a.K, a.E);
         return MPK_ERR_UNSUPPORTED;
     }
-    const int smem = C::smem_bytes(a.E);
+    const int64_t units = device_sm_count() / C::kCtas;  // tiles at once
+    const int rows = C::kWgrad ? kMaxRows
+                               : std::min(kMaxRows, (a.M + C::kRowStep - 1) / C::kRowStep * C::kRowStep);
+    p.slot_bytes = P_BYTES + rows / C::kCtas * kRowBytes;
+    // Fewer tiles than SMs: share each tile's reduction among the CTAs of a cluster, of
+    // at most 8 CTAs, each with at least 4 stages of it.
+    p.splits = 1;
+    if (!C::kWgrad && 2 * tiles <= units)
+        p.splits = (int)std::max<int64_t>(
+            1, std::min<int64_t>({units / tiles, 8 / C::kCtas, (int64_t)p.num_kb / 4}));
+    p.acc_cols = pow2_at_least(rows);
+    p.tmem_cols = p.splits > 1 ? p.acc_cols : 2 * p.acc_cols;
+    // Splits join a tile's sums in shared memory: up to 32 KiB behind the ring, else in the
+    // ring's place, whose 6 slots or more of 16 KiB + rows * 64 bytes hold the
+    // splits * ceil(rows / splits) * 512 bytes for every rows up to 256.
+    const int parts = p.splits > 1 ? (rows + p.splits - 1) / p.splits * p.splits * kCols * 4 : 0;
+    p.parts_in_ring = parts > 32768;
+    p.parts_offset = (control_bytes(a.E) + 15) / 16 * 16;
+    const int control = p.parts_offset + (p.parts_in_ring ? 0 : parts);
+    p.stages = std::min(kMaxStages, (kSmemMax - 1024 - control) / p.slot_bytes);
+    const int smem = p.stages * p.slot_bytes + control + 1024;
     const auto kernel = product_kernel<C>;
     {
         std::lock_guard<std::mutex> lk(g_attr_mu);
         if (!attr_set[dev]) {
-            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       C::smem_bytes(kMaxGroups));
+            const cudaError_t e =
+                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
             if (e != cudaSuccess) {
                 set_last_error("cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
                 return (int)e;
@@ -686,17 +845,18 @@ int launch_config(const ProductArgs& a, product::Params& p, int64_t max_tiles, c
             attr_set[dev] = true;
         }
     }
-    const int64_t units = std::min<int64_t>(tiles, device_sm_count() / C::kCtas);
+    const int ctas = C::kCtas * p.splits;
+    const int64_t grid = p.splits > 1 ? tiles : std::min(tiles, units);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)units * C::kCtas, 1, 1);
+    cfg.gridDim = dim3((unsigned)(grid * ctas), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n = 0;
-    if (C::kPair) {
+    if (ctas > 1) {
         attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 2;
+        attr[n].val.clusterDim.x = (unsigned)ctas;
         attr[n].val.clusterDim.y = 1;
         attr[n].val.clusterDim.z = 1;
         ++n;
@@ -708,19 +868,29 @@ int launch_config(const ProductArgs& a, product::Params& p, int64_t max_tiles, c
     }
     cfg.attrs = attr;
     cfg.numAttrs = (unsigned)n;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tp, tq, tq16, p);
     if (e == cudaErrorInvalidValue || e == cudaErrorLaunchOutOfResources) {
         // A context re-created by cudaDeviceReset has lost the shared-memory attribute.
         cudaGetLastError();
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem_bytes(kMaxGroups)) ==
-            cudaSuccess)
-            e = cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax) == cudaSuccess)
+            e = cudaLaunchKernelEx(&cfg, kernel, tp, tq, tq16, p);
     }
     if (e != cudaSuccess) {
         set_last_error("product launch failed: %s", cudaGetErrorString(e));
         return (int)e;
     }
     return MPK_SUCCESS;
+}
+
+template <bool kInt8, bool kPMn, bool kMx>
+int launch_rows(const ProductArgs& a, product::Params& p, cudaStream_t stream, int dev)
+{
+    using namespace product;
+    // A pair's tile has 256 columns and halves the loads of A; single CTAs give twice the
+    // tiles, for groups too small for that to matter.
+    const bool pair = (int64_t)a.M > 48 * (int64_t)a.E;
+    if (pair) return launch_config<Config<kInt8, kPMn, false, true, kMx>>(a, p, stream, dev);
+    return launch_config<Config<kInt8, kPMn, false, false, kMx>>(a, p, stream, dev);
 }
 
 }  // namespace
@@ -753,32 +923,13 @@ int launch_product(const ProductArgs& a, cudaStream_t stream)
     p.bias = a.bias;
     p.status = status;
     p.timeout_ns = wait_timeout_ns();
-    const int db = a.d_type == kTypeMxfp8 ? 1 : a.d_type == MPK_TYPE_F32 ? 4 : 2;
-    p.vec = 0;
-    for (int v : {16, 32})
-        if (reinterpret_cast<uintptr_t>(a.D) % v == 0 && a.ldd * db % v == 0) p.vec = v;
-    if (a.wgrad)
-        return launch_config<Config<false, true, true, true, 256, 6, false>>(a, p, 0, stream, dev);
-    // Tiles of 256 rows when groups have that many on average.
-    const bool pair = (int64_t)a.M >= 192 * (int64_t)a.E;
-    if (a.ab_type == kTypeInt8) {
-        if (a.b_nk) {
-            if (pair) return launch_config<Config<true, false, false, true, 256, 6, false>>(a, p, 0, stream, dev);
-            return launch_config<Config<true, false, false, false, 128, 6, false>>(a, p, 0, stream, dev);
-        }
-        if (pair) return launch_config<Config<true, false, true, true, 256, 6, false>>(a, p, 0, stream, dev);
-        return launch_config<Config<true, false, true, false, 128, 6, false>>(a, p, 0, stream, dev);
-    }
-    if (a.d_type == kTypeMxfp8) {
-        if (pair) return launch_config<Config<false, false, true, true, 256, 6, true>>(a, p, 0, stream, dev);
-        return launch_config<Config<false, false, true, false, 128, 6, true>>(a, p, 0, stream, dev);
-    }
-    if (a.b_nk) {
-        if (pair) return launch_config<Config<false, false, false, true, 256, 6, false>>(a, p, 0, stream, dev);
-        return launch_config<Config<false, false, false, false, 128, 6, false>>(a, p, 0, stream, dev);
-    }
-    if (pair) return launch_config<Config<false, false, true, true, 256, 6, false>>(a, p, 0, stream, dev);
-    return launch_config<Config<false, false, true, false, 128, 6, false>>(a, p, 0, stream, dev);
+    if (a.wgrad) return launch_config<Config<false, true, true, true, false>>(a, p, stream, dev);
+    if (a.ab_type == kTypeInt8)
+        return a.b_nk ? launch_rows<true, false, false>(a, p, stream, dev)
+                      : launch_rows<true, true, false>(a, p, stream, dev);
+    if (a.d_type == kTypeMxfp8) return launch_rows<false, true, true>(a, p, stream, dev);
+    return a.b_nk ? launch_rows<false, false, false>(a, p, stream, dev)
+                  : launch_rows<false, true, false>(a, p, stream, dev);
 }
 
 }  // namespace mpk
