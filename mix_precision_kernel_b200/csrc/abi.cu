@@ -774,7 +774,7 @@ static int run_product(ProductArgs a, cudaStream_t st)
     const int64_t per = 16 / eb;
     const int64_t b_rows = a.wgrad ? a.M : (int64_t)a.E * (a.b_nk ? a.N : a.K);
     const int64_t b_cols = a.wgrad || !a.b_nk ? a.N : a.K;
-    const bool copy_a = !none && !product_tma_ok(a.A, a.lda, eb);
+    const bool copy_a = !none && !a.x && !product_tma_ok(a.A, a.lda, eb);
     const bool copy_b = !none && !product_tma_ok(a.B, a.ldb, eb);
     if (!copy_a && !copy_b) return launch_product(a, st);
     const int64_t lda = (a.K + per - 1) / per * per, ldb = (b_cols + per - 1) / per * per;
@@ -887,6 +887,10 @@ int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int
     if (int rc = check_matrix("x", 1, M, K, ldx, type_bytes(x_type))) return rc;
     if (int rc = check_aligned(x, type_bytes(x_type), nullptr)) return rc;
     if (int rc = check_arch()) return rc;
+    if (product_quantizes(M, K)) {
+        a.x = x, a.ldx = ldx, a.x_type = x_type;
+        return run_product(a, st);
+    }
     void* ws = nullptr;
     if (int rc = take_workspace(scales_at + 4u * (size_t)M, st, &ws)) return rc;
     int8_t* codes = static_cast<int8_t*>(ws);

@@ -122,6 +122,9 @@ struct ProductArgs {
     const float* bias;       // int8 only: [N] or null
     const int32_t* offsets;  // [E + 1] on the device; null: one group of all rows (E == 1)
     int E, M, N, K;
+    const void* x;           // int8 only: A and a_scales are made from x [M][K] (rows ldx apart) on the way
+    int64_t ldx;
+    int x_type;
     bool wgrad;
     bool after_kernel;       // launched right behind a kernel of this library that allows dependents
 };
@@ -129,6 +132,8 @@ constexpr int kTypeInt8 = 16, kTypeMxfp8 = 17;
 constexpr int kMaxGroups = 1024;
 // Operands TMA can read in place: base and row strides multiples of 16 bytes.
 bool product_tma_ok(const void* p, int64_t ld, int elem_bytes);
+// Whether launch_product can quantize M rows of K itself (ProductArgs::x).
+bool product_quantizes(int M, int K);
 int launch_product(const ProductArgs& a, cudaStream_t stream);
 
 // Device-side status word of the GEMM kernels (gemm.cu): read and clear.
