@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "int8_codes.cuh"
 #include "mpk.h"
@@ -20,124 +21,211 @@ namespace cg = cooperative_groups;
 using namespace int8;
 
 // ------------------------------- rows ---------------------------------------
-// One block per row (the grid strides over the rows): a pass for the largest
-// magnitude, a pass for the codes, which finds the row in L1 or L2.
-constexpr int kRowThreads = 256;
+// kPerRow threads hold a row in registers, up to kHold 16-byte pieces each, all loaded
+// before the first is used: one pass over x.  Rows that do not fit, or whose addresses
+// allow no 16-byte pieces, are read twice, the second time from L1 or L2.
+constexpr int kRowThreads = 256, kHold = 16;
 
-template <class D, bool kVector>
+template <class D, int kPerRow, bool kVector>
 __global__ void __launch_bounds__(kRowThreads)
 int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8_t* __restrict__ codes,
                           int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K)
 {
     allow_dependent_launch();
+    constexpr int kRows = kRowThreads / kPerRow;  // of a block
     __shared__ uint32_t warp_max[kRowThreads / 32];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x % kPerRow;
     const int64_t nvec = kVector ? K / D::kVec : 0;
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-        const typename D::T* row = x + m * ldx;
-        int8_t* out = codes + m * ld_codes;
+    const bool held = nvec <= (int64_t)kPerRow * kHold;  // the same for every row
+    for (int64_t m0 = (int64_t)blockIdx.x * kRows; m0 < M; m0 += (int64_t)gridDim.x * kRows) {
+        const int64_t m = m0 + threadIdx.x / kPerRow;
+        const bool have = m < M;
+        const typename D::T* row = x + (have ? m : 0) * ldx;
+        int8_t* out = codes + (have ? m : 0) * ld_codes;
         uint32_t amax = 0;
-        for (int64_t i = tid; i < nvec; i += kRowThreads) {
-            float v[D::kVec];
-            D::widen(__ldg(reinterpret_cast<const uint4*>(row) + i), v);
+        uint4 h[kHold];
+        if (held) {
 #pragma unroll
-            for (int j = 0; j < D::kVec; ++j) amax = max(amax, magnitude(v[j]));
+            for (int j = 0; j < kHold; ++j) {
+                if (j * kPerRow >= nvec) break;
+                const int64_t i = (int64_t)j * kPerRow + tid;
+                h[j] = have && i < nvec ? __ldg(reinterpret_cast<const uint4*>(row) + i) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int j = 0; j < kHold; ++j) {
+                if (j * kPerRow >= nvec) break;
+                amax = max(amax, largest(D(), h[j]));
+            }
+        } else if (have) {
+            for (int64_t i = tid; i < nvec; i += kPerRow)
+                amax = max(amax, largest(D(), __ldg(reinterpret_cast<const uint4*>(row) + i)));
         }
-        for (int64_t k = nvec * D::kVec + tid; k < K; k += kRowThreads) amax = max(amax, magnitude(D::widen(row[k])));
+        if (have)
+            for (int64_t k = nvec * D::kVec + tid; k < K; k += kPerRow)
+                amax = max(amax, magnitude(D::widen(row[k])));
         amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-        if ((tid & 31) == 0) warp_max[tid >> 5] = amax;
-        __syncthreads();
+        if constexpr (kPerRow > 32) {
+            if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kRowThreads / 32; ++w) amax = max(amax, warp_max[w]);
-        const RowScale rs = row_scale(amax);
-        if (tid == 0) scales[m] = rs.scale;
-        for (int64_t i = tid; i < nvec; i += kRowThreads) {
-            float v[D::kVec];
-            D::widen(__ldg(reinterpret_cast<const uint4*>(row) + i), v);
-#pragma unroll
-            for (int j = 0; j < D::kVec; j += 4)
-                *reinterpret_cast<uint32_t*>(out + i * D::kVec + j) = pack4(v + j, rs.inv);
+            for (int w = 0; w < kRowThreads / 32; ++w) amax = max(amax, warp_max[w]);
         }
-        for (int64_t k = nvec * D::kVec + tid; k < K; k += kRowThreads)
-            out[k] = rs.inv == 0.0f ? (int8_t)0 : (int8_t)code_bits(D::widen(row[k]), rs.inv);
-        __syncthreads();  // warp_max is read before the next row writes it
+        const RowScale rs = row_scale(amax);
+        if (have) {
+            if (tid == 0) scales[m] = rs.scale;
+            const auto put = [&](int64_t i, const uint4& q) {
+                float v[D::kVec];
+                D::widen(q, v);
+                if constexpr (D::kVec == 8)
+                    *reinterpret_cast<uint2*>(out + i * 8) = make_uint2(pack4(v, rs.inv), pack4(v + 4, rs.inv));
+                else
+                    *reinterpret_cast<uint32_t*>(out + i * 4) = pack4(v, rs.inv);
+            };
+            if (held) {
+#pragma unroll
+                for (int j = 0; j < kHold; ++j) {
+                    if (j * kPerRow >= nvec) break;
+                    const int64_t i = (int64_t)j * kPerRow + tid;
+                    if (i < nvec) put(i, h[j]);
+                }
+            } else {
+                for (int64_t i = tid; i < nvec; i += kPerRow) put(i, __ldg(reinterpret_cast<const uint4*>(row) + i));
+            }
+            for (int64_t k = nvec * D::kVec + tid; k < K; k += kPerRow)
+                out[k] = rs.inv == 0.0f ? (int8_t)0 : (int8_t)code_bits(D::widen(row[k]), rs.inv);
+        }
+        if constexpr (kPerRow > 32) __syncthreads();  // warp_max is read before the next row writes it
     }
 }
 
 // ------------------------------ columns -------------------------------------
-// A cluster of kColCtas blocks per strip of columns and expert: each block takes a
-// share of the rows, the strip's largest magnitudes are joined through distributed
-// shared memory, and a second pass over the share (found in L2) makes the codes.
-constexpr int kColThreads = 256, kColCtas = 8;
+// A cluster of blocks per strip of columns and expert: each block takes a share of the
+// rows, the strip's largest magnitudes are joined through distributed shared memory, and
+// a second pass over the share makes the codes.  The second pass finds the share in L2 on
+// the block's own side of the chip; two kernels with the maxima in memory between them,
+// or a share held in registers, took as long or longer (4096 x 12288 BF16: 37 us, 4.1
+// TB/s of the least bytes; 44 and 52 us).
+constexpr int kColThreads = 256;
+constexpr int kColBatch = 8;   // rows a thread has in flight
+constexpr int kColBlocks = 3;  // resident blocks per SM
 
 template <class D, bool kVector>
-__global__ void __launch_bounds__(kColThreads)
+struct Cols {
+    static constexpr int V = kVector ? D::kVec : 1;
+    static constexpr int kAcross = 16;  // threads across a strip
+    static constexpr int kStrip = kAcross * V;
+    static constexpr int kDown = kColThreads / kAcross;  // rows per step
+    using Piece = std::conditional_t<kVector, uint4, typename D::T>;
+    // use(row, piece) for this thread's rows of [k0, k1), kColBatch loads at a time.
+    template <class F>
+    static __device__ __forceinline__ void each(const typename D::T* col, int64_t ldw, int64_t k0, int64_t k1, F use)
+    {
+        int64_t k = k0;
+        for (; k + (kColBatch - 1) * kDown < k1; k += kColBatch * kDown) {
+            Piece q[kColBatch];
+#pragma unroll
+            for (int i = 0; i < kColBatch; ++i)
+                q[i] = __ldg(reinterpret_cast<const Piece*>(col + (k + i * kDown) * ldw));
+#pragma unroll
+            for (int i = 0; i < kColBatch; ++i) use(k + i * kDown, q[i]);
+        }
+        for (; k < k1; k += kDown) use(k, __ldg(reinterpret_cast<const Piece*>(col + k * ldw)));
+    }
+};
+
+template <class D, bool kVector>
+__global__ void __launch_bounds__(kColThreads, kColBlocks)
 int8_quantize_cols_kernel(const typename D::T* __restrict__ w, int64_t ldw, int8_t* __restrict__ codes,
                           int64_t ld_codes, float* __restrict__ scales, int64_t K, int64_t N)
 {
-    constexpr int V = kVector ? D::kVec : 1;
-    constexpr int kAcross = kVector ? 128 / D::kVec : 32;  // threads across the strip
-    constexpr int kStrip = kAcross * V;
-    constexpr int kDown = kColThreads / kAcross;           // rows per step
-    __shared__ uint32_t smax[kStrip];
-    __shared__ float sinv[kStrip];
+    using S = Cols<D, kVector>;
+    constexpr int V = S::V;
+    constexpr bool kPacked = V == 8;  // two 16-bit magnitudes compared at once
+    constexpr int kMax = kPacked ? 4 : V;
+    __shared__ uint32_t smax[S::kStrip];
+    __shared__ float sinv[S::kStrip];
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x;
-    const int tx = tid % kAcross, ty = tid / kAcross;
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, tx = tid % S::kAcross, ty = tid / S::kAcross;
     const int64_t e = blockIdx.y;
-    const int rank = blockIdx.x % kColCtas;
-    const int64_t n0 = (int64_t)(blockIdx.x / kColCtas) * kStrip;
-    const int64_t n = n0 + tx * V;
-    const int64_t share = (K + kColCtas - 1) / kColCtas;
+    const int64_t n0 = (int64_t)(blockIdx.x / ctas) * S::kStrip, n = n0 + tx * V;
+    const int64_t share = (K + ctas - 1) / ctas;
     const int64_t k0 = min(K, rank * share), k1 = min(K, k0 + share);
-    const typename D::T* src = w + e * K * ldw;
-    int8_t* dst = codes + e * K * ld_codes;
-    for (int i = tid; i < kStrip; i += kColThreads) smax[i] = 0u;
+    const typename D::T* src = w + e * K * ldw + n;
+    const bool have = n < N;  // the vector form has N a multiple of V
+    for (int i = tid; i < S::kStrip; i += kColThreads) smax[i] = 0u;
     __syncthreads();
-    uint32_t amax[V];
+    uint32_t m[kMax];
 #pragma unroll
-    for (int j = 0; j < V; ++j) amax[j] = 0u;
-    if (n < N) {  // the vector form has N a multiple of V
-        for (int64_t k = k0 + ty; k < k1; k += kDown) {
-            float v[V];
-            if constexpr (kVector) D::widen(__ldg(reinterpret_cast<const uint4*>(src + k * ldw + n)), v);
-            else v[0] = D::widen(src[k * ldw + n]);
+    for (int j = 0; j < kMax; ++j) m[j] = 0u;
+    if (have)
+        S::each(src, ldw, k0 + ty, k1, [&](int64_t, const typename S::Piece& q) {
+            if constexpr (kPacked) {
+                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int j = 0; j < V; ++j) amax[j] = max(amax[j], magnitude(v[j]));
+                for (int j = 0; j < 4; ++j) m[j] = __vmaxu2(m[j], u[j] & 0x7FFF7FFFu);
+            } else if constexpr (kVector) {
+                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m[j] = max(m[j], u[j] & 0x7FFFFFFFu);
+            } else {
+                m[0] = max(m[0], magnitude(D::widen(q)));
+            }
+        });
+#pragma unroll
+    for (int j = 0; j < kMax; ++j) {
+        if constexpr (kPacked) {  // widened, magnitudes still order as integers
+            atomicMax(&smax[tx * V + 2 * j], magnitude(D::widen((uint16_t)m[j])));  // a maximum has no order
+            atomicMax(&smax[tx * V + 2 * j + 1], magnitude(D::widen((uint16_t)(m[j] >> 16))));
+        } else {
+            atomicMax(&smax[tx * V + j], m[j]);
         }
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) atomicMax(&smax[tx * V + j], amax[j]);  // a maximum has no order
     cluster.sync();
-    for (int i = tid; i < kStrip; i += kColThreads) {
+    for (int i = tid; i < S::kStrip; i += kColThreads) {
         uint32_t a = 0u;
-        for (int r = 0; r < kColCtas; ++r) a = max(a, *cluster.map_shared_rank(&smax[i], r));
+        for (int r = 0; r < ctas; ++r) a = max(a, *cluster.map_shared_rank(&smax[i], r));
         const RowScale rs = row_scale(a);
         sinv[i] = rs.inv;
         if (rank == 0 && n0 + i < N) scales[e * N + n0 + i] = rs.scale;
     }
     cluster.sync();  // also: no block leaves while another reads its smax
-    if (n >= N) return;
+    if (!have) return;
     float inv[V];
+    bool finite = true;  // all of this thread's columns
 #pragma unroll
-    for (int j = 0; j < V; ++j) inv[j] = sinv[tx * V + j];
-    for (int64_t k = k0 + ty; k < k1; k += kDown) {
-        float v[V];
-        if constexpr (kVector) D::widen(__ldg(reinterpret_cast<const uint4*>(src + k * ldw + n)), v);
-        else v[0] = D::widen(src[k * ldw + n]);
-        uint32_t b[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) b[j] = inv[j] == 0.0f ? 0u : code_bits(v[j], inv[j]);
-        int8_t* out = dst + k * ld_codes + n;
-        if constexpr (kVector) {
-#pragma unroll
-            for (int j = 0; j < V; j += 4)
-                *reinterpret_cast<uint32_t*>(out + j) =
-                    __byte_perm(__byte_perm(b[j], b[j + 1], 0x0040), __byte_perm(b[j + 2], b[j + 3], 0x0040), 0x5410);
-        } else {
-            *out = (int8_t)b[0];
-        }
+    for (int j = 0; j < V; ++j) {
+        inv[j] = sinv[tx * V + j];
+        finite = finite && inv[j] != 0.0f;
     }
+    int8_t* dst = codes + e * K * ld_codes + n;
+    const auto make = [&](auto all_finite) {
+        S::each(src, ldw, k0 + ty, k1, [&](int64_t k, const typename S::Piece& q) {
+            float v[V];
+            if constexpr (kVector) D::widen(q, v);
+            else v[0] = D::widen(q);
+            uint32_t c[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                c[j] = code_bits(v[j], inv[j]);
+                if (!decltype(all_finite)::value && inv[j] == 0.0f) c[j] = 0u;
+            }
+            int8_t* out = dst + k * ld_codes;
+            if constexpr (kVector) {
+                uint32_t u[V / 4];
+#pragma unroll
+                for (int j = 0; j < V; j += 4)
+                    u[j / 4] = __byte_perm(__byte_perm(c[j], c[j + 1], 0x0040),
+                                           __byte_perm(c[j + 2], c[j + 3], 0x0040), 0x5410);
+                if constexpr (V == 8) *reinterpret_cast<uint2*>(out) = make_uint2(u[0], u[1]);
+                else *reinterpret_cast<uint32_t*>(out) = u[0];
+            } else {
+                *out = (int8_t)c[0];
+            }
+        });
+    };
+    if (finite) make(std::true_type());
+    else make(std::false_type());
 }
 
 bool aligned(const void* p, int64_t ld_bytes, int to)
@@ -150,11 +238,15 @@ cudaError_t rows(const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, fl
                  cudaStream_t stream)
 {
     const auto* in = static_cast<const typename D::T*>(x);
-    const unsigned grid = (unsigned)std::min<int64_t>(M, (int64_t)device_sm_count() * 8);
-    if (aligned(x, ldx * (int64_t)sizeof(typename D::T), 16) && aligned(codes, ld_codes, 4))
-        int8_quantize_rows_kernel<D, true><<<grid, kRowThreads, 0, stream>>>(in, ldx, codes, ld_codes, scales, M, K);
-    else
-        int8_quantize_rows_kernel<D, false><<<grid, kRowThreads, 0, stream>>>(in, ldx, codes, ld_codes, scales, M, K);
+    const bool vec = aligned(x, ldx * (int64_t)sizeof(typename D::T), 16) && aligned(codes, ld_codes, D::kVec);
+    // A warp per row where rows are many and a warp can hold one; else a block per row.
+    const bool warps = M >= 4 * (int64_t)device_sm_count() && K <= (int64_t)32 * kHold * D::kVec;
+    const int64_t per_block = warps ? kRowThreads / 32 : 1;
+    const unsigned grid = (unsigned)std::min<int64_t>((M + per_block - 1) / per_block, (int64_t)device_sm_count() * 16);
+    const auto kernel = warps ? (vec ? int8_quantize_rows_kernel<D, 32, true> : int8_quantize_rows_kernel<D, 32, false>)
+                              : (vec ? int8_quantize_rows_kernel<D, kRowThreads, true>
+                                     : int8_quantize_rows_kernel<D, kRowThreads, false>);
+    kernel<<<grid, kRowThreads, 0, stream>>>(in, ldx, codes, ld_codes, scales, M, K);
     return cudaGetLastError();
 }
 
@@ -164,18 +256,19 @@ cudaError_t cols(const void* w, int64_t ldw, int8_t* codes, int64_t ld_codes, fl
 {
     const auto* in = static_cast<const typename D::T*>(w);
     const bool vec = N % D::kVec == 0 && aligned(w, ldw * (int64_t)sizeof(typename D::T), 16) &&
-                     aligned(codes, ld_codes, 4);
-    const int64_t strip = vec ? 128 : 32;
+                     aligned(codes, ld_codes, D::kVec);
+    const int64_t strip = vec ? Cols<D, true>::kStrip : Cols<D, false>::kStrip;
     const auto kernel = vec ? int8_quantize_cols_kernel<D, true> : int8_quantize_cols_kernel<D, false>;
+    constexpr unsigned kCtas = 8;
     constexpr int64_t kMaxGridY = 65535;
     for (int64_t e = 0; e < E; e += kMaxGridY) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)((N + strip - 1) / strip) * kColCtas, (unsigned)std::min(kMaxGridY, E - e));
+        cfg.gridDim = dim3((unsigned)((N + strip - 1) / strip) * kCtas, (unsigned)std::min(kMaxGridY, E - e));
         cfg.blockDim = dim3(kColThreads);
         cfg.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = kColCtas;
+        attr[0].val.clusterDim.x = kCtas;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;

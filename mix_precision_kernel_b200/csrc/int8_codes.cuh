@@ -89,5 +89,23 @@ struct F16 {
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
+// FP32 bits of the largest magnitude of a 16-byte piece.  16-bit magnitudes order as
+// integers too (NaN above infinity), so two are compared at once and the larger widened.
+__device__ __forceinline__ uint32_t largest(F32, const uint4& q)
+{
+    return max(max(q.x & 0x7FFFFFFFu, q.y & 0x7FFFFFFFu), max(q.z & 0x7FFFFFFFu, q.w & 0x7FFFFFFFu));
+}
+__device__ __forceinline__ uint32_t largest16(const uint4& q)
+{
+    const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu),
+                                __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFFu, m >> 16);
+}
+__device__ __forceinline__ uint32_t largest(Bf16, const uint4& q) { return largest16(q) << 16; }
+__device__ __forceinline__ uint32_t largest(F16, const uint4& q)
+{
+    return __float_as_uint(__half2float(__ushort_as_half((uint16_t)largest16(q)))) & 0x7FFFFFFFu;
+}
+
 }  // namespace int8
 }  // namespace mpk

@@ -54,6 +54,7 @@ namespace product {
 constexpr int kCols = 128;          // columns of D per CTA: tensor-memory lanes
 constexpr int kMaxRows = 256;       // rows of D per tile: tensor-memory columns of an accumulator
 constexpr int kRowBytes = 128;      // reduction bytes per stage
+constexpr int kTurnStride = 36;     // floats between the rows of a turned 32 x 32 chunk
 constexpr int kMaxStages = 12;
 constexpr int kEpilogueWarps = 8;
 constexpr int kFirstEpiWarp = 4;    // warps: 0 TMA, 1 MMA, 2 tail rows, 3 idle, 4-11 epilogue
@@ -97,6 +98,7 @@ struct Params {
     uint8_t* D;          // element size from d_type
     int64_t ldd, d_group;  // row and group stride of D, in elements (d_group: weight gradient)
     int d_type;
+    int d_vec;           // MXFP8: rows of D are 16-byte aligned
     uint8_t* D_scales;
     int nblkN;
     const float* a_scales;
@@ -371,7 +373,7 @@ struct Column {
         return __uint_as_float(raw);
     }
 
-    // One MX block of row `row`: the 32 lanes of the warp call it together with
+    // One MX block of row `row` held by the 32 lanes of the warp, which call it together with
     // neighbouring columns, the first a multiple of 32.  The framework's block rule, as in
     // the MXFP8 GEMM's epilogue: NaN does not enter the block's amax; columns past N are
     // zeros or NaN.
@@ -384,6 +386,47 @@ struct Column {
         const float q = v * inv;
         if (ok) p.D[row * p.ldd + n] = (uint8_t)f32x2_to_e4m3x2(q, q);
         if ((n & 31) == 0 && ok) p.D_scales[row * p.nblkN + n / 32] = (uint8_t)s;
+    }
+
+    // The MX blocks of `count` rows, raw[i] being this column's sum in row row0 + i.  A block's
+    // amax and scale are the work of one lane: the warp turns its 32 x 32 sums in shared
+    // memory (rows kTurnStride floats apart: reads and writes free of bank conflicts), so
+    // that lane i holds row i.
+    __device__ __forceinline__ void store_mx_rows(const uint32_t (&raw)[32], int count, int64_t row0, float* turn) const
+    {
+        const int lane = threadIdx.x & 31;
+        __syncwarp();  // the previous chunk has been read
+#pragma unroll
+        for (int i = 0; i < 32; ++i) turn[i * kTurnStride + lane] = __uint_as_float(raw[i]);
+        __syncwarp();
+        if (lane >= count) return;
+        const int col0 = n - lane, valid = min(32, p.N - col0);
+        float v[32], amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(turn + lane * kTurnStride + i);
+            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));
+        float inv;
+        const uint32_t s = mx_block_scale(amax, inv);
+        uint4 w[2];
+        const uint2 q0 = quantize8(v, inv), q1 = quantize8(v + 8, inv);
+        const uint2 q2 = quantize8(v + 16, inv), q3 = quantize8(v + 24, inv);
+        w[0] = make_uint4(q0.x, q0.y, q1.x, q1.y);
+        w[1] = make_uint4(q2.x, q2.y, q3.x, q3.y);
+        uint8_t* dst = p.D + (row0 + lane) * p.ldd + col0;
+        if (valid == 32 && p.d_vec) {
+            reinterpret_cast<uint4*>(dst)[0] = w[0];
+            reinterpret_cast<uint4*>(dst)[1] = w[1];
+        } else {
+            const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i < valid) dst[i] = (uint8_t)(u[i / 4] >> (8 * (i & 3)));
+        }
+        p.D_scales[(row0 + lane) * p.nblkN + col0 / 32] = (uint8_t)s;
     }
 
     template <int kType>
@@ -759,9 +802,9 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                     }
                     const int count = min(32, x.rows - c);
                     if constexpr (C::kMx) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i < count) col.store_mx(row0 + c + i, __uint_as_float(raw[i]));  // warp-uniform
+                        col.store_mx_rows(raw, count, row0 + c,
+                                          reinterpret_cast<float*>(control + p.parts_offset) +
+                                              (warp - kFirstEpiWarp) * 32 * kTurnStride);
                     } else {
                         if constexpr (C::kInt8) {
                             __syncwarp();
@@ -1013,7 +1056,8 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
     const int parts = p.splits > 1 ? ((rows + 3) / 4 + p.splits - 1) / p.splits * p.splits * 4 * kCols * 4 : 0;
     p.parts_in_ring = parts > 32768;
     p.parts_offset = (control_bytes(a.E) + 15) / 16 * 16;
-    const int behind = p.codes_bytes + p.parts_offset + (p.parts_in_ring ? 0 : parts) + 1024;
+    const int turn = C::kMx && p.splits == 1 ? kEpilogueWarps * 32 * kTurnStride * 4 : 0;
+    const int behind = p.codes_bytes + p.parts_offset + (p.parts_in_ring ? 0 : parts) + turn + 1024;
     p.ring_bytes = std::min(kMaxStages * stage_bytes<C>(rows), (kSmemMax - behind) / 1024 * 1024);
     const int ctas = C::kCtas * p.splits;
     const int64_t grid = p.splits > 1 ? tiles : std::min(tiles, units);
@@ -1084,6 +1128,7 @@ int launch_product(const ProductArgs& a, cudaStream_t stream)
     p.ldd = a.ldd;
     p.d_group = (int64_t)a.K * a.ldd;
     p.d_type = a.d_type;
+    p.d_vec = reinterpret_cast<uintptr_t>(a.D) % 16 == 0 && a.ldd % 16 == 0;
     p.D_scales = a.D_scales;
     p.nblkN = (a.N + 31) / 32;
     p.a_scales = a.a_scales;
