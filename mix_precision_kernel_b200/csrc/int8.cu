@@ -31,6 +31,10 @@ __global__ void __launch_bounds__(kRowThreads)
 int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8_t* __restrict__ codes,
                           int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K)
 {
+    // Started while the kernel in front may still run.  The product that follows may in turn
+    // load its weights once every block is past this wait: nothing in front of this kernel
+    // can be writing them then.
+    wait_for_prerequisite_grid();
     allow_dependent_launch();
     constexpr int kRows = kRowThreads / kPerRow;  // of a block
     __shared__ uint32_t warp_max[kRowThreads / 32];
@@ -246,8 +250,16 @@ cudaError_t rows(const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, fl
     const auto kernel = warps ? (vec ? int8_quantize_rows_kernel<D, 32, true> : int8_quantize_rows_kernel<D, 32, false>)
                               : (vec ? int8_quantize_rows_kernel<D, kRowThreads, true>
                                      : int8_quantize_rows_kernel<D, kRowThreads, false>);
-    kernel<<<grid, kRowThreads, 0, stream>>>(in, ldx, codes, ld_codes, scales, M, K);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = stream_captures(stream) ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, in, ldx, codes, ld_codes, scales, M, K);
 }
 
 template <class D>

@@ -98,6 +98,11 @@ int kernel_device_context(int& dev, int** status);
 int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int rank, const uint64_t* dims,
                       const uint64_t* strides_bytes, const uint32_t* box);
 
+// Whether `stream` is being captured (or cannot be asked).  Kernels that wait for the one in
+// front themselves are launched early only outside captures: in a graph that kernel may
+// be any node, or several.
+bool stream_captures(cudaStream_t stream);
+
 // int8 quantizers (int8.cu).  `type` is an MPK_TYPE_* value; arguments are validated
 // by the ABI layer.
 cudaError_t launch_int8_quantize_rows(const void* x, int type, int64_t ldx, int8_t* codes, int64_t ld_codes,

@@ -86,6 +86,7 @@ struct Params {
     int num_kb;          // rows product: stages of the reduction
     int num_n_tiles;
     int splits;          // CTAs (pairs) of a cluster that share a tile's reduction
+    int early;           // the kernel in front writes nothing but Q and its scales
     int ring_bytes;      // the ring; stage_bytes of the widest tile cuts it into stages
     int parts_in_ring, parts_offset;  // splits: where their sums meet (offset from the barriers)
     // Fused quantizer: x [M][K], and the bytes its codes take behind the ring.
@@ -163,7 +164,7 @@ struct Tile {
 // rows are cut into equal tiles of at most kMaxRows.
 template <class C>
 struct Walk {
-    static constexpr int kPanel = 8;
+    static constexpr int kPanel = 16;
     int t, stride, e = 0;
     __device__ __forceinline__ Walk(int first, int step) : t(first), stride(step) {}
     __device__ __forceinline__ bool next(const Params& p, const Table& tab, Tile& x)
@@ -533,6 +534,11 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
         }
     }
     int* widest = reinterpret_cast<int*>(control + kMiscOffset + 12);
+    // Launched to start while the kernel in front of it still runs: nothing global is touched
+    // before that one has completed, except what it is known not to write (p.early).  The
+    // next kernel may start likewise, on the SMs that this one's blocks leave first.
+    allow_dependent_launch();
+    if (!p.early) wait_for_prerequisite_grid();
     build_table<C>(p, t_lo, t_hi, t_first, scratch, widest);
     tc_fence_before();
     __syncthreads();
@@ -589,12 +595,12 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                     for (; i < mine; i += 16) load(dst + i * kRowBytes, &tmap_q16, k, x.lo + r + i);
                 }
             };
-            // The kernel in front of this one (if it allowed this one to start early) makes
-            // Q, never P: the first stages' P loads run under it.
+            // A quantizer or pre-pass in front (p.early) makes Q, never P or the groups: the
+            // first stages' P loads run under it.
             const bool have = walk.next(p, tab, x);
             int k0 = 0, k1 = 0, early = 0;
             if (have) walk.stages(p, x, split, k0, k1);
-            if (!C::kWgrad && have) {
+            if (!C::kWgrad && have && p.early) {
                 early = min(S, k1 - k0);
                 for (int i = 0; i < early; ++i) {
                     if (rank == 0)
@@ -1064,7 +1070,8 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
     cfg.gridDim = dim3((unsigned)(grid * ctas), 1, 1);
     cfg.dynamicSmemBytes = (size_t)(p.ring_bytes + behind);
     set_cluster(ctas);
-    if (a.after_kernel) {
+    p.early = a.after_kernel;
+    if (a.after_kernel || !stream_captures(stream)) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
         ++cfg.numAttrs;
@@ -1100,6 +1107,16 @@ int launch_rows(const ProductArgs& a, product::Params& p, cudaStream_t stream, i
 }
 
 }  // namespace
+
+bool stream_captures(cudaStream_t stream)
+{
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {
+        cudaGetLastError();
+        return true;
+    }
+    return status != cudaStreamCaptureStatusNone;
+}
 
 // Rows this few are quantized by the product's own CTAs, each for itself, if the codes of
 // their whole reduction leave room for the ring.
