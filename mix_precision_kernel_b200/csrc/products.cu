@@ -99,7 +99,7 @@ struct Params {
     uint8_t* D;          // element size from d_type
     int64_t ldd, d_group;  // row and group stride of D, in elements (d_group: weight gradient)
     int d_type;
-    int d_vec;           // MXFP8: rows of D are 16-byte aligned
+    int d_vec;           // MXFP8: rows of D are 16-byte aligned; 16-bit D: 4-byte aligned
     uint8_t* D_scales;
     int nblkN;
     const float* a_scales;
@@ -138,8 +138,11 @@ struct Table {
 template <class C>
 __host__ __device__ __forceinline__ int tile_width(int rows)
 {
-    const int mt = (rows + kMaxRows - 1) / kMaxRows;
-    return ((rows + mt - 1) / mt + C::kRowStep - 1) / C::kRowStep * C::kRowStep;
+    if (rows > kMaxRows) {
+        const int mt = (rows + kMaxRows - 1) / kMaxRows;
+        rows = (rows + mt - 1) / mt;
+    }
+    return (rows + C::kRowStep - 1) / C::kRowStep * C::kRowStep;
 }
 
 // Stage of a product whose widest tile has `width` rows.  The groups' real sizes decide
@@ -158,6 +161,11 @@ struct Tile {
     int width;      // rows rounded up to what the MMA takes
     int n0;         // first column
 };
+
+// ceil(2^32 / h) for the row tiles h of a panel.
+__constant__ const uint32_t kReciprocal[17] = {
+    0u,          0u,          0x80000000u, 0x55555556u, 0x40000000u, 0x33333334u, 0x2AAAAAABu, 0x24924925u, 0x20000000u,
+    0x1C71C71Du, 0x1999999Au, 0x1745D175u, 0x15555556u, 0x13B13B14u, 0x12492493u, 0x11111112u, 0x10000000u};
 
 // The tiles of one cluster: t, t + stride, ... in group order, row tiles fastest within
 // panels of kPanel, so that the tiles in flight share rows and columns in L2.  A group's
@@ -178,11 +186,16 @@ struct Walk {
         const int rows = C::kWgrad ? p.out_rows : x.hi - x.lo;
         const int mt = (rows + kMaxRows - 1) / kMaxRows;
         const int per = C::kWgrad ? kMaxRows : tile_width<C>(rows);
-        const int per_panel = kPanel * p.num_n_tiles;
-        const int panel = r / per_panel;
-        const int q = r - panel * per_panel;
-        const int h = min(kPanel, mt - panel * kPanel);
-        const int nt = q / h;
+        // The epilogue of a short reduction waits for this: no division where there is one
+        // panel (the usual case), and one by h as a multiplication, exact below 2^28.
+        int panel = 0, q = r, h = mt;
+        if (mt > kPanel) {
+            const int per_panel = kPanel * p.num_n_tiles;
+            panel = r / per_panel;
+            q = r - panel * per_panel;
+            h = min(kPanel, mt - panel * kPanel);
+        }
+        const int nt = h == 1 ? q : (int)__umulhi((uint32_t)q, kReciprocal[h]);
         x.n0 = nt * kCols * C::kCtas;
         x.r0 = (panel * kPanel + q - nt * h) * per;
         x.rows = min(per, rows - x.r0);
@@ -438,12 +451,43 @@ struct Column {
         else *reinterpret_cast<__half*>(at) = __float2half_rn(v);
     }
 
+    template <int kType>
+    __device__ __forceinline__ static uint32_t pack(float lo, float hi)
+    {
+        uint32_t r;
+        if constexpr (kType == MPK_TYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+
     // `count` rows of this column, `at` the first one's element and `step` bytes between
-    // them; sa: the rows' scales in shared memory (int8).
+    // them; sa: the rows' scales in shared memory (int8).  Warp-uniform in count.
+    // Whole chunks of a 16-bit D: neighbouring lanes swap halves of two rows' packed values,
+    // so that the even lane stores the upper row's two columns and the odd lane the lower
+    // row's, 4 bytes each.  Half the stores of one element at a time, which they were bound
+    // by (32 rows x 32 columns BF16: 674 clocks that way).
     template <int kType>
     __device__ __forceinline__ void store_rows(const uint32_t (&raw)[32], int count, uint8_t* at, int64_t step,
                                                const float* sa) const
     {
+        const int lane = threadIdx.x & 31;
+        if (kType != MPK_TYPE_F32 && count == 32 && p.d_vec && n - lane + 32 <= p.N) {
+            const uint32_t pick = (lane & 1) != 0 ? 0x3276u : 0x5410u;
+            uint8_t* to = (lane & 1) != 0 ? at - 2 + step : at;
+            const int64_t two = 2 * step;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if constexpr (C::kInt8) s = *reinterpret_cast<const float4*>(sa + i);
+                const uint32_t a = pack<kType>(value(raw[i + 0], s.x), value(raw[i + 1], s.y));
+                const uint32_t b = pack<kType>(value(raw[i + 2], s.z), value(raw[i + 3], s.w));
+                *reinterpret_cast<uint32_t*>(to) = __byte_perm(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1), pick);
+                to += two;
+                *reinterpret_cast<uint32_t*>(to) = __byte_perm(b, __shfl_xor_sync(0xFFFFFFFFu, b, 1), pick);
+                to += two;
+            }
+            return;
+        }
         if (!ok) return;
         if (count == 32) {
 #pragma unroll
@@ -1097,7 +1141,7 @@ int launch_rows(const ProductArgs& a, product::Params& p, cudaStream_t stream, i
     // A pair's tile has 256 columns and halves the loads of A; single CTAs give twice the
     // tiles, for groups too small for that to matter and for products of few tiles.
     const int64_t row_tiles = (int64_t)a.M / kMaxRows + std::min(a.E, a.M);
-    const bool pair = (int64_t)a.M > 48 * (int64_t)a.E &&
+    const bool pair = (int64_t)a.M > 48 * (int64_t)a.E && a.N > kCols &&
                       row_tiles * ((a.N + 2 * kCols - 1) / (2 * kCols)) * 4 > device_sm_count();
     if constexpr (kInt8) {
         if (a.x) return launch_config<Config<true, kPMn, false, false, false, true>>(a, p, stream, dev);
@@ -1145,7 +1189,8 @@ int launch_product(const ProductArgs& a, cudaStream_t stream)
     p.ldd = a.ldd;
     p.d_group = (int64_t)a.K * a.ldd;
     p.d_type = a.d_type;
-    p.d_vec = reinterpret_cast<uintptr_t>(a.D) % 16 == 0 && a.ldd % 16 == 0;
+    p.d_vec = a.d_type == kTypeMxfp8 ? reinterpret_cast<uintptr_t>(a.D) % 16 == 0 && a.ldd % 16 == 0
+                                     : reinterpret_cast<uintptr_t>(a.D) % 4 == 0 && a.ldd % 2 == 0;
     p.D_scales = a.D_scales;
     p.nblkN = (a.N + 31) / 32;
     p.a_scales = a.a_scales;
