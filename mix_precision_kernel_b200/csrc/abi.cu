@@ -928,7 +928,11 @@ int mpk_gemm_grouped_mxfp8(const uint8_t* A_data, const uint8_t* A_scales, const
     if (int rc = take_workspace((size_t)M * (size_t)a.lda * 2u, st, &ws)) return rc;
     a.A = ws;
     a.after_kernel = true;
-    int rc = from_cuda(launch_mxfp8_dequantize_bf16(A_data, A_scales, ws, M, K, a.lda, st), "A pre-pass launch");
+    // The codec's pre-pass for rows of whole MX blocks, the product's own for others.
+    const bool whole = K % 32 == 0 && reinterpret_cast<uintptr_t>(A_data) % 8 == 0;
+    int rc = from_cuda(whole ? launch_mxfp8_dequantize_bf16(A_data, A_scales, ws, M, K, a.lda, st)
+                             : launch_mxfp8_unpack_rows(A_data, A_scales, ws, M, K, a.lda, st),
+                       "A pre-pass launch");
     if (!rc) rc = run_product(a, st);
     const cudaError_t fe = cudaFreeAsync(ws, st);
     return rc ? rc : from_cuda(fe, "workspace release");

@@ -22,14 +22,14 @@ using namespace int8;
 
 // ------------------------------- rows ---------------------------------------
 // kPerRow threads hold a row in registers, up to kHold 16-byte pieces each, all loaded
-// before the first is used: one pass over x.  Rows that do not fit, or whose addresses
-// allow no 16-byte pieces, are read twice, the second time from L1 or L2.
+// before the first is used: one pass over x.  Longer rows are read twice, the second time
+// from L1 or L2.
 constexpr int kRowThreads = 256, kHold = 16;
 
-template <class D, int kPerRow, bool kVector>
+template <class D, int kPerRow>
 __global__ void __launch_bounds__(kRowThreads)
 int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8_t* __restrict__ codes,
-                          int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K)
+                          int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K, int)
 {
     // Started while the kernel in front may still run.  The product that follows may in turn
     // load its weights once every block is past this wait: nothing in front of this kernel
@@ -39,7 +39,7 @@ int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8
     constexpr int kRows = kRowThreads / kPerRow;  // of a block
     __shared__ uint32_t warp_max[kRowThreads / 32];
     const int tid = threadIdx.x % kPerRow;
-    const int64_t nvec = kVector ? K / D::kVec : 0;
+    const int64_t nvec = K / D::kVec;
     const bool held = nvec <= (int64_t)kPerRow * kHold;  // the same for every row
     for (int64_t m0 = (int64_t)blockIdx.x * kRows; m0 < M; m0 += (int64_t)gridDim.x * kRows) {
         const int64_t m = m0 + threadIdx.x / kPerRow;
@@ -97,6 +97,114 @@ int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8
             }
             for (int64_t k = nvec * D::kVec + tid; k < K; k += kPerRow)
                 out[k] = rs.inv == 0.0f ? (int8_t)0 : (int8_t)code_bits(D::widen(row[k]), rs.inv);
+        }
+        if constexpr (kPerRow > 32) __syncthreads();  // warp_max is read before the next row writes it
+    }
+}
+
+// Rows that do not start on a 16-byte boundary are still read in aligned pieces: piece i
+// holds elements i * kVec - off ..., off being the row's distance from the boundary before
+// it, and elements outside the row count as zeros.  The codes of piece i and the next one,
+// shifted against each other by off bytes, make output word i.  Such rows are read twice,
+// a warp each where there are many.
+constexpr int kShiftedBatch = 4;  // pieces in flight per thread
+
+template <class D>
+__device__ __forceinline__ uint4 shifted_piece(const typename D::T* row, int64_t k, int64_t K)
+{
+    if (k >= 0 && k + D::kVec <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    constexpr int kBits = 8 * sizeof(typename D::T), kPer = 32 / kBits;
+#pragma unroll
+    for (int j = 0; j < D::kVec; ++j)
+        if (k + j >= 0 && k + j < K) {
+            uint32_t e;
+            if constexpr (sizeof(typename D::T) == 4) e = __float_as_uint(row[k + j]);
+            else e = row[k + j];
+            w[j / kPer] |= e << (kBits * (j % kPer));
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The codes of a piece, the first in the lowest byte.
+template <class D>
+__device__ __forceinline__ uint64_t piece_codes(const uint4& q, float inv)
+{
+    float v[D::kVec];
+    D::widen(q, v);
+    uint64_t c = pack4(v, inv);
+    if constexpr (D::kVec == 8) c |= (uint64_t)pack4(v + 4, inv) << 32;
+    return c;
+}
+
+template <class D, int kPerRow>
+__global__ void __launch_bounds__(kRowThreads)
+int8_quantize_shifted_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8_t* __restrict__ codes,
+                          int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K, int words_ok)
+{
+    wait_for_prerequisite_grid();
+    allow_dependent_launch();
+    constexpr int V = D::kVec;
+    constexpr int kRows = kRowThreads / kPerRow;  // of a block
+    __shared__ uint32_t warp_max[kRowThreads / 32];
+    const int tid = threadIdx.x % kPerRow;
+    for (int64_t m0 = (int64_t)blockIdx.x * kRows; m0 < M; m0 += (int64_t)gridDim.x * kRows) {
+        const int64_t m = m0 + threadIdx.x / kPerRow;
+        const bool have = m < M;
+        const typename D::T* row = x + (have ? m : 0) * ldx;
+        int8_t* out = codes + (have ? m : 0) * ld_codes;
+        const int off = (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(typename D::T));
+        const int64_t nvec = (off + K + V - 1) / V;
+        const auto piece = [&](int64_t i) { return shifted_piece<D>(row, i * V - off, K); };
+        uint32_t amax = 0;
+        if (have) {
+            for (int64_t j = tid; j < nvec; j += kShiftedBatch * kPerRow) {
+                uint4 q[kShiftedBatch];
+#pragma unroll
+                for (int u = 0; u < kShiftedBatch; ++u)
+                    q[u] = j + u * kPerRow < nvec ? piece(j + u * kPerRow) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int u = 0; u < kShiftedBatch; ++u) amax = max(amax, largest(D(), q[u]));
+            }
+        }
+        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+        if constexpr (kPerRow > 32) {
+            if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kRowThreads / 32; ++w) amax = max(amax, warp_max[w]);
+        }
+        const RowScale rs = row_scale(amax);
+        if (have && tid == 0) scales[m] = rs.scale;
+        // Output word i, the codes of elements i * V .. (V of them, fewer at the row's end); all
+        // lanes of a warp call it together.  Words go out whole where the codes' rows allow.
+        const auto put = [&](int64_t i, const uint4& q) {
+            uint64_t c = piece_codes<D>(q, rs.inv);
+            uint64_t next = __shfl_down_sync(0xFFFFFFFFu, c, 1);
+            if (off != 0) {
+                if ((threadIdx.x & 31) == 31) next = have ? piece_codes<D>(piece(i + 1), rs.inv) : 0u;
+                c = (c >> (8 * off)) | (next << (8 * (V - off)));
+            }
+            const int64_t left = have ? K - i * V : 0;
+            if (left <= 0) return;
+            if (words_ok && left >= V) {
+                if constexpr (V == 8)
+                    *reinterpret_cast<uint2*>(out + i * 8) = make_uint2((uint32_t)c, (uint32_t)(c >> 32));
+                else
+                    *reinterpret_cast<uint32_t*>(out + i * 4) = (uint32_t)c;
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j < left) out[i * V + j] = (int8_t)(c >> (8 * j));
+            }
+        };
+        for (int64_t j = tid; j - tid < nvec; j += kShiftedBatch * kPerRow) {  // warp-uniform: put shuffles
+            uint4 q[kShiftedBatch];
+#pragma unroll
+            for (int u = 0; u < kShiftedBatch; ++u)
+                q[u] = have && j + u * kPerRow < nvec ? piece(j + u * kPerRow) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int u = 0; u < kShiftedBatch; ++u) put(j + u * kPerRow, q[u]);
         }
         if constexpr (kPerRow > 32) __syncthreads();  // warp_max is read before the next row writes it
     }
@@ -242,14 +350,15 @@ cudaError_t rows(const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, fl
                  cudaStream_t stream)
 {
     const auto* in = static_cast<const typename D::T*>(x);
-    const bool vec = aligned(x, ldx * (int64_t)sizeof(typename D::T), 16) && aligned(codes, ld_codes, D::kVec);
+    const int words_ok = aligned(codes, ld_codes, D::kVec);
+    const bool vec = words_ok && aligned(x, ldx * (int64_t)sizeof(typename D::T), 16);
     // A warp per row where rows are many and a warp can hold one; else a block per row.
-    const bool warps = M >= 4 * (int64_t)device_sm_count() && K <= (int64_t)32 * kHold * D::kVec;
+    const bool warps = M >= 4 * (int64_t)device_sm_count() && (!vec || K <= (int64_t)32 * kHold * D::kVec);
     const int64_t per_block = warps ? kRowThreads / 32 : 1;
     const unsigned grid = (unsigned)std::min<int64_t>((M + per_block - 1) / per_block, (int64_t)device_sm_count() * 16);
-    const auto kernel = warps ? (vec ? int8_quantize_rows_kernel<D, 32, true> : int8_quantize_rows_kernel<D, 32, false>)
-                              : (vec ? int8_quantize_rows_kernel<D, kRowThreads, true>
-                                     : int8_quantize_rows_kernel<D, kRowThreads, false>);
+    const auto kernel = vec ? (warps ? int8_quantize_rows_kernel<D, 32> : int8_quantize_rows_kernel<D, kRowThreads>)
+                            : (warps ? int8_quantize_shifted_rows_kernel<D, 32>
+                                     : int8_quantize_shifted_rows_kernel<D, kRowThreads>);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kRowThreads);
@@ -259,7 +368,7 @@ cudaError_t rows(const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, fl
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = stream_captures(stream) ? 0 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, in, ldx, codes, ld_codes, scales, M, K);
+    return cudaLaunchKernelEx(&cfg, kernel, in, ldx, codes, ld_codes, scales, M, K, words_ok);
 }
 
 template <class D>

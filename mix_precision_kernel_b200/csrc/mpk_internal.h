@@ -135,6 +135,10 @@ struct ProductArgs {
 };
 constexpr int kTypeInt8 = 16, kTypeMxfp8 = 17;
 constexpr int kMaxGroups = 1024;
+// MXFP8 [M][K] -> BF16 rows ld_out apart (a multiple of 8; out 16-byte aligned), any K and
+// alignment; elements between K and the next multiple of 8 become zeros.
+cudaError_t launch_mxfp8_unpack_rows(const uint8_t* data, const uint8_t* scales, void* out, int64_t M, int64_t K,
+                                     int64_t ld_out, cudaStream_t stream);
 // Operands TMA can read in place: base and row strides multiples of 16 bytes.
 bool product_tma_ok(const void* p, int64_t ld, int elem_bytes);
 // Whether launch_product can quantize M rows of K itself (ProductArgs::x).

@@ -413,8 +413,8 @@ struct Column {
 #pragma unroll
         for (int i = 0; i < 32; ++i) turn[i * kTurnStride + lane] = __uint_as_float(raw[i]);
         __syncwarp();
-        if (lane >= count) return;
         const int col0 = n - lane, valid = min(32, p.N - col0);
+        const bool whole = valid == 32 && p.d_vec;
         float v[32], amax = 0.0f;
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -431,16 +431,24 @@ struct Column {
         w[0] = make_uint4(q0.x, q0.y, q1.x, q1.y);
         w[1] = make_uint4(q2.x, q2.y, q3.x, q3.y);
         uint8_t* dst = p.D + (row0 + lane) * p.ldd + col0;
-        if (valid == 32 && p.d_vec) {
-            reinterpret_cast<uint4*>(dst)[0] = w[0];
-            reinterpret_cast<uint4*>(dst)[1] = w[1];
-        } else {
-            const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i < valid) dst[i] = (uint8_t)(u[i / 4] >> (8 * (i & 3)));
+        if (lane < count) {
+            p.D_scales[(row0 + lane) * p.nblkN + col0 / 32] = (uint8_t)s;
+            if (whole) {
+                reinterpret_cast<uint4*>(dst)[0] = w[0];
+                reinterpret_cast<uint4*>(dst)[1] = w[1];
+            }
         }
-        p.D_scales[(row0 + lane) * p.nblkN + col0 / 32] = (uint8_t)s;
+        if (whole) return;
+        // Ragged or unaligned rows: turned back, so that the warp stores one row at a time.
+        __syncwarp();
+        uint4* mine = reinterpret_cast<uint4*>(turn + lane * kTurnStride);
+        mine[0] = w[0];
+        mine[1] = w[1];
+        __syncwarp();
+        if (lane >= valid) return;
+        uint8_t* to = p.D + row0 * p.ldd + n;
+        for (int i = 0; i < count; ++i, to += p.ldd)
+            *to = reinterpret_cast<const uint8_t*>(turn + i * kTurnStride)[lane];
     }
 
     template <int kType>
@@ -983,6 +991,46 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
     }
 }
 
+// MXFP8 rows -> BF16 rows padded to a multiple of 8 elements, for a K or an alignment that the
+// codec's kernel takes element by element: a warp per row, 8 codes per lane and step from
+// two aligned 8-byte words (the granules that hold them lie within the codes).
+constexpr int kUnpackThreads = 256;
+
+__global__ void __launch_bounds__(kUnpackThreads)
+mxfp8_unpack_rows_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
+                         uint16_t* __restrict__ out, int64_t M, int64_t K, int64_t ld_out)
+{
+    wait_for_prerequisite_grid();
+    allow_dependent_launch();
+    const int lane = threadIdx.x & 31;
+    const int64_t nblk = (K + 31) / 32, warps = (int64_t)gridDim.x * (kUnpackThreads / 32);
+    for (int64_t m = (int64_t)blockIdx.x * (kUnpackThreads / 32) + threadIdx.x / 32; m < M; m += warps) {
+        const uint8_t* row = data + m * K;
+        for (int64_t k = 8 * lane; k < K; k += 256) {
+            const uint8_t* at = row + k;
+            const uint8_t* word = at - (reinterpret_cast<uintptr_t>(at) & 7u);
+            const int shift = 8 * (int)(at - word);
+            uint64_t c;
+            if (k + 8 <= K && word >= data && word + 16 <= data + M * K) {
+                c = __ldg(reinterpret_cast<const unsigned long long*>(word));
+                if (shift != 0)
+                    c = (c >> shift) | ((uint64_t)__ldg(reinterpret_cast<const unsigned long long*>(word) + 1) << (64 - shift));
+            } else {
+                c = 0u;
+                for (int j = 0; j < 8 && k + j < K; ++j) c |= (uint64_t)row[k + j] << (8 * j);
+            }
+            const float s = e8m0_to_f32(scales[m * nblk + k / 32]);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = e4m3x2_to_f32x2((uint32_t)(c >> (16 * j)) & 0xFFFFu);
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(f.y * s), "f"(f.x * s));
+            }
+            *reinterpret_cast<uint4*>(out + m * ld_out + k) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
 }  // namespace product
 
 // ----------------------------------------------------------------------------
@@ -1151,6 +1199,25 @@ int launch_rows(const ProductArgs& a, product::Params& p, cudaStream_t stream, i
 }
 
 }  // namespace
+
+cudaError_t launch_mxfp8_unpack_rows(const uint8_t* data, const uint8_t* scales, void* out, int64_t M, int64_t K,
+                                     int64_t ld_out, cudaStream_t stream)
+{
+    using namespace product;
+    if (M == 0 || K == 0) return cudaSuccess;
+    const int64_t blocks = std::min<int64_t>((M + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32),
+                                             (int64_t)device_sm_count() * 8);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kUnpackThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = stream_captures(stream) ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, mxfp8_unpack_rows_kernel, data, scales, static_cast<uint16_t*>(out), M, K, ld_out);
+}
 
 bool stream_captures(cudaStream_t stream)
 {
