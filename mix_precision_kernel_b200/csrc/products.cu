@@ -206,13 +206,13 @@ struct Walk {
     // Stages [k0, k1) of a tile's reduction that split s of p.splits takes.
     __device__ __forceinline__ static void stages(const Params& p, const Tile& x, int s, int& k0, int& k1)
     {
-        if constexpr (C::kWgrad) {
-            k0 = 0;
-            k1 = (x.hi - x.lo + C::BK - 1) / C::BK;
-        } else {
-            k0 = (int)((int64_t)p.num_kb * s / p.splits);
-            k1 = (int)((int64_t)p.num_kb * (s + 1) / p.splits);
-        }
+        const int n = all_stages(p, x);
+        k0 = p.splits == 1 ? 0 : (int)((int64_t)n * s / p.splits);
+        k1 = p.splits == 1 ? n : (int)((int64_t)n * (s + 1) / p.splits);
+    }
+    __device__ __forceinline__ static int all_stages(const Params& p, const Tile& x)
+    {
+        return C::kWgrad ? (x.hi - x.lo + C::BK - 1) / C::BK : p.num_kb;
     }
     // Weight gradient: rows of the last stage that belong to the group, 0 if no row
     // behind them needs zeroing (an MMA takes 16 rows, and MMAs past the end are left out).
@@ -672,7 +672,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                     }
                     uint32_t bar;
                     last_tail &= ~(1u << s);
-                    if (C::kWgrad && tail_rows > 0 && kb == k1 - 1) {
+                    if (C::kWgrad && tail_rows > 0 && kb == walk.all_stages(p, x) - 1) {
                         // This CTA's tail warp takes the stage first.
                         bar = tail(s);
                         last_tail |= 1u << s;
@@ -738,7 +738,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                         break;
                     }
                     int steps = 4;
-                    if (C::kWgrad && kb == k1 - 1 && rem != 0) {
+                    if (C::kWgrad && rem != 0 && kb == walk.all_stages(p, x) - 1) {
                         steps = (rem + 15) / 16;
                         fence_acq_rel_cluster();  // the tail warps' zeros, of both CTAs
                     }
@@ -776,7 +776,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
         while (ok && walk.next(p, tab, x)) {
             int k0, k1;
             walk.stages(p, x, split, k0, k1);
-            const int rows = walk.tail_rows(x);
+            const int rows = k1 == walk.all_stages(p, x) ? walk.tail_rows(x) : 0;  // another split has the last stage
             if (k1 == k0) continue;
             const int last = (s + k1 - k0 - 1) % S;
             s = (last + 1) % S;
@@ -891,7 +891,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
     }
     __syncwarp();
 
-    if (!C::kWgrad && p.splits > 1 && unit < tab.first[p.E]) {
+    if (p.splits > 1 && unit < tab.first[p.E]) {
         // Join the splits' sums in their order.  Block g of four rows is finished by split
         // g % splits: every CTA hands its part of the block to that split's CTA of the same
         // columns, as block g / splits of slice `split` there ([block][column][4 rows]).
@@ -900,7 +900,10 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
         const int ew = warp - kFirstEpiWarp;
         const int quad = warp & 3, turn = ew / 4;
         const int blocks = (x.rows + 3) / 4, share = (blocks + p.splits - 1) / p.splits;
-        const int64_t row0 = (int64_t)x.lo + x.r0;
+        const int64_t row0 = C::kWgrad ? (int64_t)x.r0 : (int64_t)x.lo + x.r0;
+        const int64_t base0 = C::kWgrad ? x.e * p.d_group : 0;
+        int k0, k1;
+        again.stages(p, x, split, k0, k1);  // a short group may leave this split nothing
         const Column<C> col(p, x, x.n0 + kCols * (int)rank + quad * 32 + lane);
         const bool busy = ew >= 0 && col.n - lane < p.N;
         // Slices lie in the ring's place if there is no room behind it: then every CTA's
@@ -923,8 +926,13 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
 #pragma unroll 1
             for (int c = 32 * turn; c < x.rows; c += 64) {
                 uint32_t raw[32];
-                tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
-                tmem_ld_wait();
+                if (k1 > k0) {
+                    tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) raw[i] = 0u;
+                }
                 int to = (c / 4) % p.splits, block = (c / 4) / p.splits;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
@@ -963,7 +971,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                     if constexpr (C::kMx) {
                         col.store_mx(row, d);
                     } else if (col.ok) {
-                        uint8_t* at = p.D + (row * p.ldd + col.n) * (p.d_type == MPK_TYPE_F32 ? 4 : 2);
+                        uint8_t* at = p.D + (base0 + row * p.ldd + col.n) * (p.d_type == MPK_TYPE_F32 ? 4 : 2);
                         if (p.d_type == MPK_TYPE_BF16) col.template put<MPK_TYPE_BF16>(at, d);
                         else if (p.d_type == MPK_TYPE_F16) col.template put<MPK_TYPE_F16>(at, d);
                         else col.template put<MPK_TYPE_F32>(at, d);
@@ -1124,8 +1132,9 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
     // Fewer tiles than SMs: share each tile's reduction among the CTAs of a cluster, of
     // at most 8 CTAs, each with at least 4 stages of it, if all clusters can run at once.
     p.splits = 1;
-    if (!C::kWgrad && 2 * tiles <= units) {
-        int most = (int)std::min<int64_t>({units / tiles, 8 / C::kCtas, (int64_t)p.num_kb / 4});
+    if (2 * tiles <= units) {
+        const int64_t stages = C::kWgrad ? (int64_t)a.M / a.E / C::BK : p.num_kb;
+        int most = (int)std::min<int64_t>({units / tiles, 8 / C::kCtas, stages / 4});
         for (; most > 1; --most) {
             const int ctas = C::kCtas * most;
             int& n = max_clusters[dev][ctas];

@@ -481,3 +481,65 @@ def test_experts_forward_and_backward_together(mpk_lib, cuda):
     H64 = torch.cat([x[lo:lo + n].double() @ w1[e].double()
                      for e, (lo, n) in enumerate(zip(np.concatenate([[0], np.cumsum(sizes)]).tolist(), sizes))])
     assert float((m.dequantize(hd, hs).double() - H64).norm() / H64.norm()) <= 2 * 2.0 ** -4
+
+
+@pytest.mark.parametrize("sizes", [[3000], [1000, 0, 3, 2500], [2048, 64, 17, 1], [4097]], ids=str)
+@pytest.mark.parametrize("N,K", [(64, 72), (200, 371), (256, 256)])
+def test_long_groups_with_small_weights(mpk_lib, cuda, sizes, N, K):
+    """Few tiles and a long ragged reduction: it is shared by a cluster, of which short and
+    empty groups leave some blocks nothing."""
+    import torch
+
+    m = mpk_lib
+    gen = torch.Generator(device="cuda").manual_seed(N + len(sizes))
+    M = sum(sizes) + 5
+    for dtype, out in ((torch.bfloat16, torch.float32), (torch.float16, torch.float16)):
+        A, G = _ints((M, K), gen, dtype, 8, span=1), _ints((M, N), gen, dtype, 8, span=1)
+        A[M - 5:] = float("nan")
+        G[M - 5:] = float("nan")
+        _equal(m.gemm_grouped_wgrad(A, G, _offsets(sizes), out), _wgrad_64(A, G, sizes), out)
+    assert m.device_status() == 0
+
+
+def test_operands_written_just_before(mpk_lib, cuda):
+    """Back to back on one stream, without a pause: weights, codes, offsets and activations
+    are rewritten between the calls that read them, by the library's own kernels and by
+    others, and results are overwritten at once.  Every call sees its own operands."""
+    import torch
+
+    m = mpk_lib
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    E, M, K, N = 3, 64, 512, 1024
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    w = torch.empty((E, K, N), dtype=torch.bfloat16, device="cuda")
+    x = torch.empty((M, K), dtype=torch.bfloat16, device="cuda")
+    d = torch.empty((M, N), dtype=torch.float32, device="cuda")
+    q = torch.empty((M, N), dtype=torch.float32, device="cuda")
+    dw = torch.empty((E, K, N), dtype=torch.float32, device="cuda")
+    rounds = 12
+    ws = [torch.randint(-2, 3, (E, K, N), generator=gen, device="cuda").bfloat16() for _ in range(rounds)]
+    xs = [torch.randint(-2, 3, (M, K), generator=gen, device="cuda").bfloat16() for _ in range(rounds)]
+    splits = [[0, 10 + i, 30 + i, M] for i in range(rounds)]
+    offs = [torch.tensor(s, dtype=torch.int32, device="cuda") for s in splits]
+    got = []
+    torch.cuda.synchronize()
+    for i in range(rounds):
+        off.copy_(offs[i])
+        w.copy_(ws[i])
+        x.copy_(xs[i])
+        m.gemm_grouped(x, w, off, out=d)
+        codes, scales = m.quantize_int8_cols(w[0])
+        m.linear_int8(x, codes, scales, out=q)
+        m.gemm_grouped_wgrad(x, d.bfloat16(), off, out=dw)
+        got.append((d.clone(), q.clone(), dw.clone()))
+    torch.cuda.synchronize()
+    for i in range(rounds):
+        sizes = np.diff(splits[i]).tolist()
+        _equal(got[i][0], _product_64(xs[i], ws[i], sizes), torch.float32)
+        c, s = m.quantize_int8_cols(ws[i][0])
+        torch.cuda.synchronize()
+        assert torch.equal(got[i][1], m.linear_int8(xs[i], c, s, out_dtype=torch.float32))
+        torch.cuda.synchronize()
+        bound = M * 2.0 ** -23 * _wgrad_64(xs[i].abs(), got[i][0].bfloat16().abs(), sizes)
+        diff = (got[i][2].double() - _wgrad_64(xs[i], got[i][0].bfloat16(), sizes)).abs()
+        assert int((diff > bound).sum()) == 0
