@@ -574,29 +574,31 @@ def _vector(t, what: str, dtype, shape: tuple, like):
 
 
 def _result(out, shape: tuple, dtype, like):
+    """(out, or a new contiguous tensor; its row stride)."""
     if out is None:
-        return like.new_empty(shape, dtype=dtype)
+        cols = shape[-1]
+        strides = (cols, 1) if len(shape) == 2 else (shape[1] * cols, cols, 1)
+        return _torch.empty_strided(shape, strides, dtype=dtype, device=like.device), cols
     if out.shape != shape or out.dtype is not dtype or out.get_device() != like.get_device():
         _want(out, "out", len(shape), dtype, shape, like)
-    return out
-
-
-def _launch(fn, like, *args):
-    """Call a C entry point on the current stream of like's device."""
-    index = like.get_device()
-    cuda = _torch.cuda
-    if cuda.current_device() == index:
-        status = fn(*args, _raw_stream(index))
-    else:
-        with cuda.device(index):
-            status = fn(*args, _raw_stream(index))
-    if status != MPK_SUCCESS:
-        _check(status)
+    return out, _row_stride(out, "out")
 
 
 def _raw_stream(index: int) -> int:
     get = getattr(_torch._C, "_cuda_getCurrentRawStream", None)
     return get(index) if get is not None else _torch.cuda.current_stream(index).cuda_stream
+
+
+def _launch(fn, like, *args):
+    """Call a C entry point on the current stream of like's device."""
+    index = like.get_device()
+    if _torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with _torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status != MPK_SUCCESS:
+        _check(status)
 
 
 def _padded_codes(shape, like):
@@ -660,10 +662,10 @@ def gemm_int8(A, A_scales, B, B_scales, bias=None, out_dtype=None, b_layout: int
         _vector(bias, "bias", torch.float32, (N,), A)
     dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
     d = _type_code(dtype, "D")
-    D = _result(out, (M, N), dtype, A)
+    D, ldd = _result(out, (M, N), dtype, A)
     _launch(lib().mpk_gemm_int8, A, A.data_ptr(), _row_stride(A, "A"), A_scales.data_ptr(), B.data_ptr(),
             _row_stride(B, "B"), b_layout, B_scales.data_ptr(), None if bias is None else bias.data_ptr(),
-            D.data_ptr(), d, _row_stride(D, "D"), M, N, K)
+            D.data_ptr(), d, ldd, M, N, K)
     return D
 
 
@@ -679,10 +681,10 @@ def linear_int8(x, B, B_scales, bias=None, out_dtype=None, b_layout: int = B_KN,
         _vector(bias, "bias", torch.float32, (N,), x)
     dtype = out_dtype or (x.dtype if out is None else out.dtype)
     d = _type_code(dtype, "D")
-    D = _result(out, (M, N), dtype, x)
+    D, ldd = _result(out, (M, N), dtype, x)
     _launch(lib().mpk_linear_int8, x, x.data_ptr(), t, _row_stride(x, "x"), B.data_ptr(), _row_stride(B, "B"),
             b_layout, B_scales.data_ptr(), None if bias is None else bias.data_ptr(), D.data_ptr(), d,
-            _row_stride(D, "D"), M, N, K)
+            ldd, M, N, K)
     return D
 
 
@@ -701,9 +703,9 @@ def gemm_grouped(A, B, offsets, out_dtype=None, b_layout: int = B_KN, out=None):
     _vector(offsets, "offsets", torch.int32, (E + 1,), A)
     dtype = out_dtype or (A.dtype if out is None else out.dtype)
     d = _type_code(dtype, "D")
-    D = _result(out, (M, N), dtype, A)
+    D, ldd = _result(out, (M, N), dtype, A)
     _launch(lib().mpk_gemm_grouped, A, A.data_ptr(), _row_stride(A, "A"), B.data_ptr(), _row_stride(B, "B"),
-            b_layout, t, D.data_ptr(), d, _row_stride(D, "D"), offsets.data_ptr(), E, M, N, K)
+            b_layout, t, D.data_ptr(), d, ldd, offsets.data_ptr(), E, M, N, K)
     return D
 
 
@@ -720,9 +722,9 @@ def gemm_grouped_int8(A, A_scales, B, B_scales, offsets, out_dtype=None, b_layou
     _vector(offsets, "offsets", torch.int32, (E + 1,), A)
     dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
     d = _type_code(dtype, "D")
-    D = _result(out, (M, N), dtype, A)
+    D, ldd = _result(out, (M, N), dtype, A)
     _launch(lib().mpk_gemm_grouped_int8, A, A.data_ptr(), _row_stride(A, "A"), A_scales.data_ptr(), B.data_ptr(),
-            _row_stride(B, "B"), b_layout, B_scales.data_ptr(), D.data_ptr(), d, _row_stride(D, "D"),
+            _row_stride(B, "B"), b_layout, B_scales.data_ptr(), D.data_ptr(), d, ldd,
             offsets.data_ptr(), E, M, N, K)
     return D
 
@@ -739,8 +741,8 @@ def gemm_grouped_mxfp8(A_data, A_scales, B, offsets, out=None):
     _vector(A_scales, "A_scales", torch.uint8, (M, nblk(K)), A_data)
     _vector(offsets, "offsets", torch.int32, (E + 1,), A_data)
     D, Ds = out if out is not None else (None, None)
-    D = _result(D, (M, N), torch.uint8, A_data)
-    Ds = _result(Ds, (M, nblk(N)), torch.uint8, A_data)
+    D, _ = _result(D, (M, N), torch.uint8, A_data)
+    Ds, _ = _result(Ds, (M, nblk(N)), torch.uint8, A_data)
     if not D.is_contiguous() or not Ds.is_contiguous():
         raise ValueError("out must be contiguous")
     _launch(lib().mpk_gemm_grouped_mxfp8, A_data, A_data.data_ptr(), A_scales.data_ptr(), B.data_ptr(),
@@ -763,7 +765,7 @@ def gemm_grouped_wgrad(A, dD, offsets, out_dtype=None, out=None):
     _vector(offsets, "offsets", torch.int32, (E + 1,), A)
     dtype = out_dtype or (A.dtype if out is None else out.dtype)
     d = _type_code(dtype, "dB")
-    dB = _result(out, (E, K, N), dtype, A)
+    dB, ldd = _result(out, (E, K, N), dtype, A)
     _launch(lib().mpk_gemm_grouped_wgrad, A, A.data_ptr(), _row_stride(A, "A"), dD.data_ptr(), _row_stride(dD, "dD"),
-            t, dB.data_ptr(), d, _row_stride(dB, "dB"), offsets.data_ptr(), E, M, N, K)
+            t, dB.data_ptr(), d, ldd, offsets.data_ptr(), E, M, N, K)
     return dB
