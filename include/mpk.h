@@ -236,10 +236,11 @@ int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int
                     void* stream);
 
 /* Products grouped by expert: rows offsets[e] <= i < offsets[e + 1] of D are the same
- * rows of A times B[e], e < E.  offsets: int32 [E + 1] in device memory, non-decreasing
- * (values outside 0..M are clamped to it, a group whose end lies before its start is
- * empty, and where groups overlap D holds either's rows).  Rows of D outside every group
- * are left as they were.  B[e] at e * K * ldb (MPK_B_KN) or e * N * ldb (MPK_B_NK); E up to
+ * rows of A times B[e], e < E.  offsets: int32 [E + 1] in device memory, non-decreasing.
+ * Values outside 0..M are clamped to it and a group whose end lies before its start is
+ * empty: no offsets lead outside the operands, but where they decrease so that groups
+ * overlap, which of these rows are computed, and with which B, is unspecified.  Rows of D
+ * outside every group are left as they were.  D must not overlap the operands.  B[e] at e * K * ldb (MPK_B_KN) or e * N * ldb (MPK_B_NK); E up to
  * MPK_MAX_GROUPS.  Nothing is copied to the host: the calls can be captured.
  *
  * mpk_gemm_grouped: A and B of the same 16-bit type (MPK_TYPE_BF16 or MPK_TYPE_F16), FP32

@@ -85,6 +85,7 @@ struct Params {
     int N;               // columns of D
     int num_kb;          // rows product: stages of the reduction
     int num_n_tiles;
+    int have_operands;   // the reduction is not empty: the operands' tensor maps are set
     int splits;          // CTAs (pairs) of a cluster that share a tile's reduction
     int early;           // the kernel in front writes nothing but Q and its scales
     int ring_bytes;      // the ring; stage_bytes of the widest tile cuts it into stages
@@ -223,8 +224,8 @@ struct Walk {
     }
 };
 
-// Groups' bounds -> the table in shared memory; returns the widest tile's rows (after a
-// __syncthreads, as the table itself).  Bounds are clamped to [0, M] and to
+// Groups' bounds -> the table in shared memory, and the widest tile's rows (both to be read
+// after a __syncthreads).  Bounds are clamped to [0, M] and to
 // non-negative lengths, so that no value of offsets leads outside the operands.
 template <class C>
 __device__ void build_table(const Params& p, int* lo, int* hi, int* first, int* scratch, int* widest)
@@ -554,7 +555,9 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
     const int split = crank / C::kCtas;
     const uint32_t leader = (uint32_t)(crank - (int)rank);
     const int unit = (int)blockIdx.x / ctas;
-    const int nunits = (int)gridDim.x / ctas;
+    // Splits: one tile per cluster, whatever the groups say (the host counted tiles of groups
+    // that do not overlap, and only one accumulator is allocated).
+    const int nunits = p.splits > 1 ? 1 << 30 : (int)gridDim.x / ctas;
 
     if (warp == 0) {
         if (lane < kMaxStages) {
@@ -571,7 +574,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
             *never_abort = 0;
         }
         fence_mbar_init();
-    } else if (warp == 3 && p.num_kb > 0) {
+    } else if (warp == 3 && p.have_operands) {
         if (lane == 0) prefetch_tmap(&tmap_p);
         if (lane == 1 && !C::kFuse) prefetch_tmap(&tmap_q);
         if (lane == 2 && !C::kWgrad && !C::kFuse) prefetch_tmap(&tmap_q16);
@@ -1068,6 +1071,7 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
                                    : a.ab_type == MPK_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const int reduction = C::kWgrad ? a.M : a.K;
+    p.have_operands = reduction > 0;
     if (reduction > 0) {  // otherwise no load is issued
         const uint64_t qdims[2] = {(uint64_t)a.K, (uint64_t)a.M};
         const uint64_t qstr[1] = {(uint64_t)a.lda * eb};
@@ -1100,8 +1104,10 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
     const int64_t row_tiles = C::kWgrad ? (int64_t)a.E * ((a.K + kMaxRows - 1) / kMaxRows)
                                         : (int64_t)a.M / kMaxRows + std::min(a.E, a.M);
     const int64_t tiles = row_tiles * p.num_n_tiles;
-    if (tiles > INT32_MAX / 16) {
-        set_last_error("product of more than 2^27 tiles (M=%d N=%d K=%d, %d groups)", a.M, a.N, a.K, a.E);
+    // Nor may groups that overlap, against the rules, count past 32 bits.
+    const int64_t most_tiles = C::kWgrad ? tiles : (int64_t)a.E * ((a.M + (int64_t)kMaxRows - 1) / kMaxRows) * p.num_n_tiles;
+    if (tiles > INT32_MAX / 16 || most_tiles > INT32_MAX / 2) {
+        set_last_error("product of too many tiles (M=%d N=%d K=%d, %d groups)", a.M, a.N, a.K, a.E);
         return MPK_ERR_UNSUPPORTED;
     }
     const int64_t units = device_sm_count() / C::kCtas;  // tiles at once

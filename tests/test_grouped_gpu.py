@@ -543,3 +543,23 @@ def test_operands_written_just_before(mpk_lib, cuda):
         bound = M * 2.0 ** -23 * _wgrad_64(xs[i].abs(), got[i][0].bfloat16().abs(), sizes)
         diff = (got[i][2].double() - _wgrad_64(xs[i], got[i][0].bfloat16(), sizes)).abs()
         assert int((diff > bound).sum()) == 0
+
+
+@pytest.mark.parametrize("M,E,K", [(1, 64, 4096), (40, 3, 2048), (300, 16, 512)])
+def test_overlapping_groups_stay_inside(mpk_lib, cuda, M, E, K):
+    """Offsets that run back and forth, so that groups overlap and there are more tiles than
+    disjoint groups could have: nothing outside the groups is written and no wait gives up."""
+    import torch
+
+    m = mpk_lib
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    rows = 8 + M
+    off = torch.tensor([0 if e % 2 == 0 else M for e in range(E + 1)], dtype=torch.int32, device="cuda")
+    A, B = _ints((rows, K), gen, torch.bfloat16, span=1), _ints((E, K, 128), gen, torch.bfloat16, span=1)
+    whole = torch.full((rows, 160), 4.0, dtype=torch.bfloat16, device="cuda")
+    m.gemm_grouped(A, B, off, out=whole[:, :128])
+    assert bool((whole[M:] == 4).all()) and bool((whole[:, 128:] == 4).all())
+    dB = m.gemm_grouped_wgrad(A, A[:, :128], off, torch.float32)
+    want = A[:M].double().t() @ A[:M, :128].double()
+    _equal(dB[0], want, torch.float32)
+    assert m.device_status() == 0

@@ -304,3 +304,45 @@ def test_streams_and_graphs(mpk_lib, cuda):
         for (gr, y, z), v in zip(graphs, want):
             assert torch.equal(y, z) and torch.equal(y, v * (1 + rep))
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 17, 700])
+def test_linear_of_unaligned_and_strided_rows(mpk_lib, cuda, dtype, M):
+    """Rows of x off a 16-byte boundary and apart, weights off it too, D odd columns wide and
+    inside a larger tensor; the same result as from contiguous operands."""
+    import torch
+
+    m = mpk_lib
+    rng = np.random.default_rng(M)
+    K, N = 333, 65
+    x = _values(rng, (M, K), "normal")
+    B, sb = m.quantize_int8_cols(_tensor(_values(rng, (K, N), "normal"), "float32"))
+    plain = m.linear_int8(_tensor(x, dtype), B, sb)
+    odd = torch.empty((K * N + 3,), dtype=torch.int8, device="cuda")[3:].view(K, N)
+    odd.copy_(B)
+    whole = torch.full((M, 2 * N + 1), 5.0, dtype=plain.dtype, device="cuda")
+    for pad, shift in ((3, 1), (8, 0), (5, 7)):
+        for w in (B, odd):
+            D = m.linear_int8(_tensor(x, dtype, pad, shift), w, sb, out=whole[:, 1:N + 1])
+            assert torch.equal(D, plain)
+            assert bool((whole[:, 0] == 5).all()) and bool((whole[:, N + 1:] == 5).all())
+    assert m.device_status() == 0
+
+
+def test_fused_and_separate_quantizers_agree(mpk_lib, cuda):
+    """Up to four rows are quantized inside the product, more in a kernel of their own: a row's
+    result does not depend on how many others come with it."""
+    import torch
+
+    m = mpk_lib
+    for K in (64, 1000, 8192, 8200, 20000):
+        x = torch.randn((9, K), device="cuda").bfloat16()
+        x[1, K // 2] = float("nan")
+        B, sb = m.quantize_int8_cols(torch.randn((K, 300), device="cuda"))
+        all_rows = m.linear_int8(x, B, sb, out_dtype=torch.float32)
+        for n in (1, 2, 3, 4):
+            got = m.linear_int8(x[:n], B, sb, out_dtype=torch.float32)
+            assert torch.equal(got.nan_to_num(7.0), all_rows[:n].nan_to_num(7.0))
+            assert torch.equal(got.isnan(), all_rows[:n].isnan())
+    assert m.device_status() == 0
