@@ -184,13 +184,28 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
         :: "r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int32_t y,
-                                            int32_t z)
+// L2 policy of data that is read once: it leaves first.
+__device__ __forceinline__ uint64_t l2_evict_first()
 {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];"
-        :: "r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
+// policy 0: the default one (a policy that says the same costs 3 % of a large product).
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int32_t y,
+                                            int32_t z, uint64_t policy)
+{
+    if (policy != 0)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+            :: "r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy) : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];"
+            :: "r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
 __device__ __forceinline__ void prefetch_tmap(const void* tmap)
@@ -416,12 +431,18 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
 }
 
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, uint32_t bar_cluster,
-                                                 int32_t x, int32_t y, int32_t z)
+                                                 int32_t x, int32_t y, int32_t z, uint64_t policy)
 {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];"
-        :: "r"(dst), "l"(tmap), "r"(bar_cluster), "r"(x), "r"(y), "r"(z) : "memory");
+    if (policy != 0)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+            :: "r"(dst), "l"(tmap), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "l"(policy) : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];"
+            :: "r"(dst), "l"(tmap), "r"(bar_cluster), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
 // Arrive on an mbarrier of a CTA of this cluster, ordering this thread's earlier
