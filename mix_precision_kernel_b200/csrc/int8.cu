@@ -28,8 +28,8 @@ constexpr int kRowThreads = 256, kHold = 16;
 
 template <class D, int kPerRow>
 __global__ void __launch_bounds__(kRowThreads)
-int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8_t* __restrict__ codes,
-                          int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K, int)
+int8_quantize_rows_kernel(const typename D::T* x, int64_t ldx, int8_t* codes,
+                          int64_t ld_codes, float* scales, int64_t M, int64_t K, int)
 {
     // Started while the kernel in front may still run.  The product that follows may in turn
     // load its weights once every block is past this wait: nothing in front of this kernel
@@ -53,7 +53,7 @@ int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8
             for (int j = 0; j < kHold; ++j) {
                 if (j * kPerRow >= nvec) break;
                 const int64_t i = (int64_t)j * kPerRow + tid;
-                h[j] = have && i < nvec ? __ldg(reinterpret_cast<const uint4*>(row) + i) : make_uint4(0u, 0u, 0u, 0u);
+                h[j] = have && i < nvec ? load_16b(reinterpret_cast<const uint4*>(row) + i) : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
             for (int j = 0; j < kHold; ++j) {
@@ -62,7 +62,7 @@ int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8
             }
         } else if (have) {
             for (int64_t i = tid; i < nvec; i += kPerRow)
-                amax = max(amax, largest(D(), __ldg(reinterpret_cast<const uint4*>(row) + i)));
+                amax = max(amax, largest(D(), load_16b(reinterpret_cast<const uint4*>(row) + i)));
         }
         if (have)
             for (int64_t k = nvec * D::kVec + tid; k < K; k += kPerRow)
@@ -93,7 +93,7 @@ int8_quantize_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8
                     if (i < nvec) put(i, h[j]);
                 }
             } else {
-                for (int64_t i = tid; i < nvec; i += kPerRow) put(i, __ldg(reinterpret_cast<const uint4*>(row) + i));
+                for (int64_t i = tid; i < nvec; i += kPerRow) put(i, load_16b(reinterpret_cast<const uint4*>(row) + i));
             }
             for (int64_t k = nvec * D::kVec + tid; k < K; k += kPerRow)
                 out[k] = rs.inv == 0.0f ? (int8_t)0 : (int8_t)code_bits(D::widen(row[k]), rs.inv);
@@ -112,7 +112,7 @@ constexpr int kShiftedBatch = 4;  // pieces in flight per thread
 template <class D>
 __device__ __forceinline__ uint4 shifted_piece(const typename D::T* row, int64_t k, int64_t K)
 {
-    if (k >= 0 && k + D::kVec <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    if (k >= 0 && k + D::kVec <= K) return load_16b(row + k);
     uint32_t w[4] = {0u, 0u, 0u, 0u};
     constexpr int kBits = 8 * sizeof(typename D::T), kPer = 32 / kBits;
 #pragma unroll
@@ -139,8 +139,8 @@ __device__ __forceinline__ uint64_t piece_codes(const uint4& q, float inv)
 
 template <class D, int kPerRow>
 __global__ void __launch_bounds__(kRowThreads)
-int8_quantize_shifted_rows_kernel(const typename D::T* __restrict__ x, int64_t ldx, int8_t* __restrict__ codes,
-                          int64_t ld_codes, float* __restrict__ scales, int64_t M, int64_t K, int words_ok)
+int8_quantize_shifted_rows_kernel(const typename D::T* x, int64_t ldx, int8_t* codes,
+                          int64_t ld_codes, float* scales, int64_t M, int64_t K, int words_ok)
 {
     wait_for_prerequisite_grid();
     allow_dependent_launch();

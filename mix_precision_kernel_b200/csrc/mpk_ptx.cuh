@@ -35,6 +35,22 @@ __device__ __forceinline__ void wait_for_prerequisite_grid()
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Loads of data that a prerequisite grid may have written, after wait_for_prerequisite_grid.
+// The read-only path (__ldg, or const __restrict__ pointers) is for data that does not
+// change while the kernel runs, and a kernel launched early runs before that wait returns.
+__device__ __forceinline__ uint4 load_16b(const void* p)
+{
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint64_t load_8b(const void* p)
+{
+    uint64_t v;
+    asm volatile("ld.global.u64 %0, [%1];" : "=l"(v) : "l"(p));
+    return v;
+}
+
 // Two E4M3 codes (low byte = first element) -> two floats, exact.
 __device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t two_codes)
 {

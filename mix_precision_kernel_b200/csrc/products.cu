@@ -319,7 +319,7 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
 #pragma unroll 4
         for (int i = start; i < nvec; i += stride) {
             float v[V];
-            T::widen(__ldg(reinterpret_cast<const uint4*>(row) + i), v);
+            T::widen(load_16b(reinterpret_cast<const uint4*>(row) + i), v);
 #pragma unroll
             for (int j = 0; j < V; ++j) a = max(a, int8::magnitude(v[j]));
         }
@@ -341,7 +341,7 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
 #pragma unroll 2
         for (int i = kfirst / V + start; i < vlast; i += stride) {
             float v[V];
-            T::widen(__ldg(reinterpret_cast<const uint4*>(row) + i), v);
+            T::widen(load_16b(reinterpret_cast<const uint4*>(row) + i), v);
             uint32_t* dst = reinterpret_cast<uint32_t*>(at(i * V));
 #pragma unroll
             for (int j = 0; j < V; j += 4) dst[j / 4] = int8::pack4(v + j, rs.inv);
@@ -1010,8 +1010,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
 constexpr int kUnpackThreads = 256;
 
 __global__ void __launch_bounds__(kUnpackThreads)
-mxfp8_unpack_rows_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
-                         uint16_t* __restrict__ out, int64_t M, int64_t K, int64_t ld_out)
+mxfp8_unpack_rows_kernel(const uint8_t* data, const uint8_t* scales, uint16_t* out, int64_t M, int64_t K, int64_t ld_out)
 {
     wait_for_prerequisite_grid();
     allow_dependent_launch();
@@ -1025,9 +1024,9 @@ mxfp8_unpack_rows_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
             const int shift = 8 * (int)(at - word);
             uint64_t c;
             if (k + 8 <= K && word >= data && word + 16 <= data + M * K) {
-                c = __ldg(reinterpret_cast<const unsigned long long*>(word));
+                c = load_8b(word);
                 if (shift != 0)
-                    c = (c >> shift) | ((uint64_t)__ldg(reinterpret_cast<const unsigned long long*>(word) + 1) << (64 - shift));
+                    c = (c >> shift) | (load_8b(word + 8) << (64 - shift));
             } else {
                 c = 0u;
                 for (int j = 0; j < 8 && k + j < K; ++j) c |= (uint64_t)row[k + j] << (8 * j);
