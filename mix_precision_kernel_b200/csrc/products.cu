@@ -1249,11 +1249,14 @@ bool stream_captures(cudaStream_t stream)
     return status != cudaStreamCaptureStatusNone;
 }
 
-// Rows this few are quantized by the product's own CTAs, each for itself, if the codes of
-// their whole reduction leave room for the ring.
-// Measured on B200 against the row quantizer in front (1 x 12288 x 4096: 13.5 against 14.5
-// us; 16 rows: 20.2 against 14.9, every CTA then reads 128 KiB of x).
-bool product_quantizes(int M, int K) { return M <= 4 && K > 0 && K <= 8192; }
+// Few rows are quantized by the product's own CTAs, each for itself, if the codes of their
+// whole reduction leave room for the ring.  Every CTA then reads all of x; against the row
+// quantizer in front, which costs a launch and a workspace, measured on B200: 1 x 4096 x 4096 9.6
+// against 12.3 us, 16 x 512 x 512 7.2 against 8.6; 4 x 12288 x 4096 14.4 against 13.5.
+bool product_quantizes(int M, int K)
+{
+    return M <= product::kFusedRows && K > 0 && (int64_t)M * K <= 8192;
+}
 
 bool product_tma_ok(const void* p, int64_t ld, int elem_bytes)
 {

@@ -331,17 +331,17 @@ def test_linear_of_unaligned_and_strided_rows(mpk_lib, cuda, dtype, M):
 
 
 def test_fused_and_separate_quantizers_agree(mpk_lib, cuda):
-    """Up to four rows are quantized inside the product, more in a kernel of their own: a row's
-    result does not depend on how many others come with it."""
+    """Few rows are quantized inside the product (up to 16 of 512, 1 of 8192), more in a kernel
+    of their own: a row's result does not depend on how many others come with it."""
     import torch
 
     m = mpk_lib
-    for K in (64, 1000, 8192, 8200, 20000):
-        x = torch.randn((9, K), device="cuda").bfloat16()
+    for K in (64, 512, 1000, 4096, 8192, 8200, 20000):
+        x = torch.randn((33, K), device="cuda").bfloat16()
         x[1, K // 2] = float("nan")
         B, sb = m.quantize_int8_cols(torch.randn((K, 300), device="cuda"))
         all_rows = m.linear_int8(x, B, sb, out_dtype=torch.float32)
-        for n in (1, 2, 3, 4):
+        for n in (1, 2, 3, 4, 7, 8, 9, 16, 17):
             got = m.linear_int8(x[:n], B, sb, out_dtype=torch.float32)
             assert torch.equal(got.nan_to_num(7.0), all_rows[:n].nan_to_num(7.0))
             assert torch.equal(got.isnan(), all_rows[:n].isnan())
