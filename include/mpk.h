@@ -1,5 +1,6 @@
 /*
- * libmpk -- C ABI of the B200 (sm_100a) MXFP8 x BF16 GEMM and MXFP8 codec.
+ * libmpk -- C ABI of the B200 (sm_100a) MXFP8 x BF16 GEMM and MXFP8 codec, and of
+ * int8 products and products grouped by expert.
  *
  * Drop-in boundary for the hot path of chcoliang/mix_precision_kernel:
  *

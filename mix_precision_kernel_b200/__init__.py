@@ -1,4 +1,4 @@
-"""B200 (sm_100a) MXFP8 x BF16 GEMM and MXFP8 codec.
+"""B200 (sm_100a) MXFP8 x BF16 GEMM, MXFP8 codec, int8 products and products grouped by expert.
 
 Python binding of ``libmpk.so`` (C ABI in ``include/mpk.h``) through ctypes.
 The function names follow the reference project's C++ API
@@ -10,6 +10,10 @@ The function names follow the reference project's C++ API
     mxfp8_dequantize_gpu(data, scales, output, M, K, stream)
     mxfp8_quantize_host(input, data, scales, M, K)
     mxfp8_dequantize_host(data, scales, output, M, K)
+
+The int8 products (``gemm_int8``, ``linear_int8``), the products grouped by expert
+(``gemm_grouped``, ``gemm_grouped_int8``, ``gemm_grouped_mxfp8``, ``gemm_grouped_wgrad``) and the
+int8 quantizers (``quantize_int8``, ``quantize_int8_cols``) have no counterpart there.
 
 Arguments are torch CUDA tensors (or raw device addresses as ints) for the GPU
 functions and numpy arrays for the host functions.  Where the reference calls

@@ -23,7 +23,8 @@ using namespace int8;
 // ------------------------------- rows ---------------------------------------
 // kPerRow threads hold a row in registers, up to kHold 16-byte pieces each, all loaded
 // before the first is used: one pass over x.  Longer rows are read twice, the second time
-// from L1 or L2.
+// from L1 or L2.  16384 x 2048 BF16 in 22.2 us (4.5 TB/s of the least bytes), 4096 x 8192 FP32
+// in 34.3 us (4.9 TB/s).
 constexpr int kRowThreads = 256, kHold = 16;
 
 template <class D, int kPerRow>
@@ -106,7 +107,7 @@ int8_quantize_rows_kernel(const typename D::T* x, int64_t ldx, int8_t* codes,
 // holds elements i * kVec - off ..., off being the row's distance from the boundary before
 // it, and elements outside the row count as zeros.  The codes of piece i and the next one,
 // shifted against each other by off bytes, make output word i.  Such rows are read twice,
-// a warp each where there are many.
+// a warp each where there are many (8846 x 4991 BF16 in 51 us; 65 us with a block per row).
 constexpr int kShiftedBatch = 4;  // pieces in flight per thread
 
 template <class D>
