@@ -708,6 +708,12 @@ static int validate_product(const ProductArgs& a, const int32_t* offsets, bool g
         set_last_error("negative size M=%d N=%d K=%d E=%d", a.M, a.N, a.K, a.E);
         return MPK_ERR_INVALID_VALUE;
     }
+    // Tiles and boxes may reach a little past the last row, column or reduction element.
+    constexpr int kMaxSize = INT32_MAX - 1023;
+    if (a.M > kMaxSize || a.N > kMaxSize || a.K > kMaxSize) {
+        set_last_error("sizes up to %d, got M=%d N=%d K=%d", kMaxSize, a.M, a.N, a.K);
+        return MPK_ERR_UNSUPPORTED;
+    }
     if (b_layout != MPK_B_KN && b_layout != MPK_B_NK) {
         set_last_error("unknown layout of B %d", b_layout);
         return MPK_ERR_INVALID_VALUE;

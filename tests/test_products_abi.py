@@ -43,6 +43,7 @@ def test_sizes_and_pointers_are_refused(mpk_lib, call):
     L = mpk_lib.lib()
     for size in ("M", "N", "K"):
         assert call(L, **{size: -1}) == INVALID
+        assert call(L, **{size: 2 ** 31 - 1}) == UNSUPPORTED
     assert call(L, B=None) == INVALID if call is not _wgrad else call(L, G=None) == INVALID
     assert call(L, D=None) == INVALID
     if call is _linear:
