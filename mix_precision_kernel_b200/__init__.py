@@ -606,21 +606,28 @@ def _launch(fn, like, *args):
 
 
 def _padded_codes(shape, like):
-    """int8 codes whose rows start on 16-byte boundaries (read in place by the products)."""
+    """int8 codes whose rows start on 16-byte boundaries (read in place by the products), and
+    their row stride."""
     ld = (shape[-1] + 15) // 16 * 16
-    codes = like.new_empty(tuple(shape[:-1]) + (ld,), dtype=_torch.int8)
-    return (codes if ld == shape[-1] else codes[..., :shape[-1]]), ld
+    strides = (ld, 1) if len(shape) == 2 else (shape[1] * ld, ld, 1)
+    return _torch.empty_strided(tuple(shape), strides, dtype=_torch.int8, device=like.device), ld
+
+
+def _scales(shape: tuple, like):
+    strides = (1,) if len(shape) == 1 else (shape[1], 1)
+    return _torch.empty_strided(shape, strides, dtype=_torch.float32, device=like.device)
 
 
 def quantize_int8(x):
     """float32, bfloat16 or float16 [M, K] -> (codes int8 [M, K], scales float32 [M]): one
     scale per row.  The codes' rows are padded to a multiple of 16 bytes."""
-    torch = _torch or _init_torch()
+    if _torch is None:
+        _init_torch()
     M, K = _matrix(x, "x", 2, None)
     t = _type_code(x.dtype, "x")
     ldx = _row_stride(x, "x")
     codes, ld = _padded_codes((M, K), x)
-    scales = x.new_empty((M,), dtype=torch.float32)
+    scales = _scales((M,), x)
     _launch(lib().mpk_int8_quantize_rows, x, x.data_ptr(), t, ldx, codes.data_ptr(), ld, scales.data_ptr(), M, K)
     return codes, scales
 
@@ -629,14 +636,15 @@ def quantize_int8_cols(w):
     """float32, bfloat16 or float16 [K, N] or [E, K, N] -> (codes int8 of the same shape,
     scales float32 [N] or [E, N]): one scale per column.  The codes' rows are padded to a
     multiple of 16 bytes."""
-    torch = _torch or _init_torch()
+    if _torch is None:
+        _init_torch()
     shape = _matrix(w, "w", 3 if w.dim() == 3 else 2, None)
     t = _type_code(w.dtype, "w")
     E = shape[0] if len(shape) == 3 else 1
     K, N = shape[-2:]
     ldw = _row_stride(w, "w")
     codes, ld = _padded_codes(shape, w)
-    scales = w.new_empty(tuple(shape[:-2]) + (N,), dtype=torch.float32)
+    scales = _scales((N,) if len(shape) == 2 else (E, N), w)
     _launch(lib().mpk_int8_quantize_cols, w, w.data_ptr(), t, ldw, codes.data_ptr(), ld, scales.data_ptr(), E, K, N)
     return codes, scales
 
