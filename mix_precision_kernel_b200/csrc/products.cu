@@ -38,7 +38,7 @@
 // against 20.6 for the bytes alone); many rows, the tensor pipe and, over seconds, the
 // power cap (int8 4096x12288x4096 in 128 us, 3.2 POP/s, the pipe busy 82 % of the time; BF16
 // with one group 262 to 269 us, 1.53 to 1.57 PFLOP/s); a short reduction, the epilogue's
-// stores (weight gradient of 32 x 2048x2816 BF16 in 123 us, 3.0 TB/s).
+// stores (weight gradient of 32 x 2048x2816 BF16 in 87 us, 4.2 TB/s).
 //
 // Every mbarrier wait is bounded (mpk::mbar_wait); on expiry the CTA raises an abort
 // flag, records a status code, drains what it has in flight and leaves.
@@ -63,9 +63,9 @@ constexpr int kMaxRows = 256;       // rows of D per tile: tensor-memory columns
 constexpr int kRowBytes = 128;      // reduction bytes per stage
 constexpr int kTurnStride = 36;     // floats between the rows of a turned 32 x 32 chunk
 constexpr int kMaxStages = 12;
-constexpr int kEpilogueWarps = 8;
-constexpr int kFirstEpiWarp = 4;    // warps: 0 TMA, 1 MMA, 2 tail rows, 3 idle, 4-11 epilogue
-constexpr int kThreads = 32 * (kFirstEpiWarp + kEpilogueWarps);
+constexpr int kFirstEpiWarp = 4;    // warps: 0 TMA, 1 MMA, 2 tail rows, 3 idle, then the epilogue's
+constexpr int kMaxWarps = 20;
+constexpr int kFuseWarps = 8;       // epilogue warps of a product that quantizes its rows
 constexpr int P_BYTES = kCols * kRowBytes;  // columns operand per CTA and stage
 constexpr uint64_t kDrainTimeoutNs = 200000000ull;
 
@@ -74,8 +74,8 @@ constexpr uint64_t kDrainTimeoutNs = 200000000ull;
 // words each).
 constexpr int kNumBars = 3 * kMaxStages + 6;
 constexpr int kMiscOffset = kNumBars * 8;
-constexpr int kScaleOffset = (kMiscOffset + 16 + 4 * 2 * (kThreads / 32) + 15) / 16 * 16;  // 32 row scales per warp
-constexpr int kCodesOffset = kScaleOffset + 32 * 4 * kEpilogueWarps;  // fused quantizer: amax and scale per row
+constexpr int kScaleOffset = (kMiscOffset + 16 + 4 * 2 * kMaxWarps + 15) / 16 * 16;  // 32 row scales per warp
+constexpr int kCodesOffset = kScaleOffset + 32 * 4 * (kMaxWarps - kFirstEpiWarp);  // fused quantizer: amax and scale per row
 constexpr int kFusedRows = 16;      // most rows of a product that quantizes them itself
 constexpr int kTableOffset = kCodesOffset + 2 * 4 * kFusedRows;
 
@@ -134,6 +134,12 @@ struct Config {
     static constexpr int kMnBox = kInt8 ? 128 : 64;   // elements across an MN-major box
     static constexpr int kBoxBytes = kRowBytes * BK;  // an MN-major box: BK rows of 128 bytes
     static constexpr int kRowStep = 16 * kCtas;       // a tile's rows are a multiple
+    // A weight gradient often has more to store than to multiply: twice the epilogue (32 x
+    // 2048x2816 BF16 of 4096 rows: 123 -> 87 us), which costs products with a long reduction
+    // 2 to 3 %.
+    static constexpr int kEpiWarps = kWgrad ? 16 : 8;
+    static constexpr int kTurns = kEpiWarps / 4;      // warps that take turns at chunks of 32 rows
+    static constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
     static constexpr int kFullArrivals = kWgrad && kPair ? 2 : 1;
 };
 
@@ -254,7 +260,7 @@ __device__ void build_table(const Params& p, int* lo, int* hi, int* first, int* 
         }
         return;
     }
-    constexpr int kPer = (kMaxGroups + kThreads - 1) / kThreads;
+    constexpr int kThreads = C::kThreads, kPer = (kMaxGroups + kThreads - 1) / kThreads;
     int count[kPer];
     int sum = 0, wide = C::kRowStep;
 #pragma unroll
@@ -304,7 +310,7 @@ __device__ void build_table(const Params& p, int* lo, int* hi, int* first, int* 
     }
 }
 
-// The fused quantizer: the epilogue warps (ew of kEpilogueWarps) make the codes of rows
+// The fused quantizer: the epilogue warps (ew of kFuseWarps) make the codes of rows
 // 0 .. M - 1 for the reduction's elements [kfirst, klast) in shared memory, as TMA would
 // have laid them out (a block of kFusedRows rows per stage, 128-byte swizzle), and the
 // rows' scales.  Every CTA reads whole rows of x for their largest magnitude, while its
@@ -319,8 +325,8 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
     const int nvec = p.x_vec ? p.K / V : 0;
     const int start = (ew % warps) * 32 + lane, stride = warps * 32;
     if (ew == 0 && lane < kFusedRows) amax_bits[lane] = 0u;
-    named_bar_sync(1, 32 * kEpilogueWarps);
-    for (int m = ew / warps; m < M; m += kEpilogueWarps / warps) {
+    named_bar_sync(1, 32 * kFuseWarps);
+    for (int m = ew / warps; m < M; m += kFuseWarps / warps) {
         const typename T::T* row = static_cast<const typename T::T*>(p.x) + m * p.ldx;
         uint32_t a = 0u;
 #pragma unroll 4
@@ -334,8 +340,8 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
         a = __reduce_max_sync(0xFFFFFFFFu, a);
         if (lane == 0) atomicMax(&amax_bits[m], a);  // a maximum has no order
     }
-    named_bar_sync(1, 32 * kEpilogueWarps);
-    for (int m = ew / warps; m < M; m += kEpilogueWarps / warps) {
+    named_bar_sync(1, 32 * kFuseWarps);
+    for (int m = ew / warps; m < M; m += kFuseWarps / warps) {
         const typename T::T* row = static_cast<const typename T::T*>(p.x) + m * p.ldx;
         const int8::RowScale rs = int8::row_scale(amax_bits[m]);
         if (start == 0) scales[m] = rs.scale;
@@ -357,7 +363,7 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
             *at(k) = rs.inv == 0.0f ? (uint8_t)0 : (uint8_t)int8::code_bits(T::widen(row[k]), rs.inv);
     }
     fence_proxy_async_smem();
-    named_bar_sync(1, 32 * kEpilogueWarps);
+    named_bar_sync(1, 32 * kFuseWarps);
 }
 
 template <class C>
@@ -525,7 +531,7 @@ struct Column {
 };
 
 template <class C>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(C::kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                const __grid_constant__ CUtensorMap tmap_q16, const Params p)
 {
@@ -574,7 +580,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
             mbar_init(tail(lane), 1);
         } else if (lane < kMaxStages + 2) {
             mbar_init(tfull(lane - kMaxStages), 1);
-            mbar_init(tempty(lane - kMaxStages), C::kCtas * kEpilogueWarps);
+            mbar_init(tempty(lane - kMaxStages), C::kCtas * C::kEpiWarps);
         } else if (lane == kMaxStages + 2) {
             mbar_init(drain, 1);
             mbar_init(codes_ready, 1);
@@ -815,7 +821,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
         }
     } else if (warp >= kFirstEpiWarp) {
         // -------------------------------- epilogue ---------------------------------
-        // Two warps per quarter of the columns take turns at chunks of 32 rows.
+        // The warps of a quarter of the columns take turns at chunks of 32 rows.
         const int quad = warp & 3;
         const int turn = (warp - kFirstEpiWarp) / 4;
         const uint32_t tempty0 = C::kPair ? mapa_shared(tempty(0), leader) : tempty(0);
@@ -846,11 +852,12 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
             const bool any = k1 > k0;  // otherwise nothing was accumulated: zeros
             const int64_t row0 = C::kWgrad ? (int64_t)x.r0 : (int64_t)x.lo + x.r0;
             const int64_t base0 = (C::kWgrad ? x.e * p.d_group : 0) + row0 * p.ldd;
-            float sa[kMaxRows / 64];  // scale of this lane's row of each chunk, under the MMAs
+            float sa[4];  // scale of this lane's row of each chunk, loaded under the MMAs
             if constexpr (C::kInt8) {
+                static_assert(!C::kInt8 || 4 * 32 * C::kTurns == kMaxRows, "four chunks per warp");
 #pragma unroll
-                for (int j = 0; j < kMaxRows / 64; ++j) {
-                    const int r = 64 * j + 32 * turn + lane;
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 32 * (C::kTurns * j + turn) + lane;
                     sa[j] = r < x.rows ? (C::kFuse ? fused_scales[r & (kFusedRows - 1)] : p.a_scales[row0 + r]) : 0.0f;
                 }
             }
@@ -861,7 +868,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
             if (warp_ok) {
                 int j = 0;
 #pragma unroll 1
-                for (int c = 32 * turn; c < x.rows; c += 64, ++j) {
+                for (int c = 32 * turn; c < x.rows; c += 32 * C::kTurns, ++j) {
                     uint32_t raw[32];
                     if (any) {
                         tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
@@ -936,7 +943,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
             const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16);
             const uint32_t mine = smem_u32(parts) + 16u * (uint32_t)(split * share * kCols + quad * 32 + lane);
 #pragma unroll 1
-            for (int c = 32 * turn; c < x.rows; c += 64) {
+            for (int c = 32 * turn; c < x.rows; c += 32 * C::kTurns) {
                 uint32_t raw[32];
                 if (k1 > k0) {
                     tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
@@ -959,7 +966,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
         cluster_sync_all();
         if (busy && *abort_flag == 0) {
             const uint4* part = reinterpret_cast<const uint4*>(parts) + quad * 32 + lane;
-            for (int j = turn; split + j * p.splits < blocks; j += 2) {
+            for (int j = turn; split + j * p.splits < blocks; j += C::kTurns) {
                 uint4 v[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
@@ -1132,7 +1139,7 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
         attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
@@ -1177,7 +1184,7 @@ int launch_config(const ProductArgs& a, product::Params& p, cudaStream_t stream,
     const int parts = p.splits > 1 ? ((rows + 3) / 4 + p.splits - 1) / p.splits * p.splits * 4 * kCols * 4 : 0;
     p.parts_in_ring = parts > 32768;
     p.parts_offset = (control_bytes(a.E) + 15) / 16 * 16;
-    const int turn = C::kMx && p.splits == 1 ? kEpilogueWarps * 32 * kTurnStride * 4 : 0;
+    const int turn = C::kMx && p.splits == 1 ? C::kEpiWarps * 32 * kTurnStride * 4 : 0;
     const int behind = p.codes_bytes + p.parts_offset + (p.parts_in_ring ? 0 : parts) + turn + 1024;
     p.ring_bytes = std::min(kMaxStages * stage_bytes<C>(rows), (kSmemMax - behind) / 1024 * 1024);
     const int ctas = C::kCtas * p.splits;
