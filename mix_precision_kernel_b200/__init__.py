@@ -412,9 +412,16 @@ def gemm_plan(M: int, N: int, K: int) -> tuple[int, int, int]:
 # int8 and expert-grouped products (tensors or device addresses; see include/mpk.h)
 # ---------------------------------------------------------------------------
 
+def _sizes(*sizes):
+    """The C entry points take sizes as 32-bit integers; ctypes would cut larger ones off."""
+    if max(sizes) > 0x7FFFFFFF or min(sizes) < -0x80000000:
+        raise ValueError(f"sizes must fit 32-bit integers, got {sizes}")
+
+
 def int8_quantize_rows_gpu(input, input_type: int, ld_input: int, codes, ld_codes: int, scales, M: int, K: int,
                            stream=None) -> None:
     """int8 codes of input [M, K] and one FP32 scale per row; row strides in elements."""
+    _sizes(M, K)
     s = _stream(stream, input, codes)
     _check(lib().mpk_int8_quantize_rows(_addr(input), input_type, ld_input, _addr(codes), ld_codes, _addr(scales),
                                         M, K, s))
@@ -423,6 +430,7 @@ def int8_quantize_rows_gpu(input, input_type: int, ld_input: int, codes, ld_code
 def int8_quantize_cols_gpu(input, input_type: int, ld_input: int, codes, ld_codes: int, scales, E: int, K: int,
                            N: int, stream=None) -> None:
     """int8 codes of input [E, K, N] and one FP32 scale per matrix and column."""
+    _sizes(E, N, K)
     s = _stream(stream, input, codes)
     _check(lib().mpk_int8_quantize_cols(_addr(input), input_type, ld_input, _addr(codes), ld_codes, _addr(scales),
                                         E, K, N, s))
@@ -431,6 +439,7 @@ def int8_quantize_cols_gpu(input, input_type: int, ld_input: int, codes, ld_code
 def gemm_int8_gpu(A, lda: int, A_scales, B, ldb: int, b_layout: int, B_scales, bias, D, d_type: int, ldd: int,
                   M: int, N: int, K: int, stream=None) -> None:
     """D = (A*B) * A_scales[row] * B_scales[column] + bias (int8 A and B; bias may be None)."""
+    _sizes(M, N, K)
     s = _stream(stream, A, D)
     _check(lib().mpk_gemm_int8(_addr(A), lda, _addr(A_scales), _addr(B), ldb, b_layout, _addr(B_scales),
                                _addr(bias), _addr(D), d_type, ldd, M, N, K, s))
@@ -439,6 +448,7 @@ def gemm_int8_gpu(A, lda: int, A_scales, B, ldb: int, b_layout: int, B_scales, b
 def linear_int8_gpu(x, x_type: int, ldx: int, B, ldb: int, b_layout: int, B_scales, bias, D, d_type: int, ldd: int,
                     M: int, N: int, K: int, stream=None) -> None:
     """gemm_int8_gpu of x quantized per row on the way."""
+    _sizes(M, N, K)
     s = _stream(stream, x, D)
     _check(lib().mpk_linear_int8(_addr(x), x_type, ldx, _addr(B), ldb, b_layout, _addr(B_scales), _addr(bias),
                                  _addr(D), d_type, ldd, M, N, K, s))
@@ -447,6 +457,7 @@ def linear_int8_gpu(x, x_type: int, ldx: int, B, ldb: int, b_layout: int, B_scal
 def gemm_grouped_gpu(A, lda: int, B, ldb: int, b_layout: int, ab_type: int, D, d_type: int, ldd: int, offsets,
                      E: int, M: int, N: int, K: int, stream=None) -> None:
     """Rows offsets[e]..offsets[e + 1] of D = the same rows of A times B[e] (16-bit types)."""
+    _sizes(E, M, N, K)
     s = _stream(stream, A, D)
     _check(lib().mpk_gemm_grouped(_addr(A), lda, _addr(B), ldb, b_layout, ab_type, _addr(D), d_type, ldd,
                                   _addr(offsets), E, M, N, K, s))
@@ -455,6 +466,7 @@ def gemm_grouped_gpu(A, lda: int, B, ldb: int, b_layout: int, ab_type: int, D, d
 def gemm_grouped_int8_gpu(A, lda: int, A_scales, B, ldb: int, b_layout: int, B_scales, D, d_type: int, ldd: int,
                           offsets, E: int, M: int, N: int, K: int, stream=None) -> None:
     """gemm_grouped_gpu of int8 codes with row scales [M] and column scales [E, N]."""
+    _sizes(E, M, N, K)
     s = _stream(stream, A, D)
     _check(lib().mpk_gemm_grouped_int8(_addr(A), lda, _addr(A_scales), _addr(B), ldb, b_layout, _addr(B_scales),
                                        _addr(D), d_type, ldd, _addr(offsets), E, M, N, K, s))
@@ -463,6 +475,7 @@ def gemm_grouped_int8_gpu(A, lda: int, A_scales, B, ldb: int, b_layout: int, B_s
 def gemm_grouped_mxfp8_gpu(A_data, A_scales, B, ldb: int, D_data, D_scales, offsets, E: int, M: int, N: int, K: int,
                            stream=None) -> None:
     """gemm_grouped_gpu with A and D in MXFP8 and B in BF16."""
+    _sizes(E, M, N, K)
     s = _stream(stream, A_data, D_data)
     _check(lib().mpk_gemm_grouped_mxfp8(_addr(A_data), _addr(A_scales), _addr(B), ldb, _addr(D_data),
                                         _addr(D_scales), _addr(offsets), E, M, N, K, s))
@@ -471,6 +484,7 @@ def gemm_grouped_mxfp8_gpu(A_data, A_scales, B, ldb: int, D_data, D_scales, offs
 def gemm_grouped_wgrad_gpu(A, lda: int, dD, ldg: int, ab_type: int, dB, d_type: int, ldd: int, offsets, E: int,
                            M: int, N: int, K: int, stream=None) -> None:
     """dB[e] [K, N] = A[rows of e]^T * dD[rows of e]; zeros for an empty group."""
+    _sizes(E, M, N, K)
     s = _stream(stream, A, dB)
     _check(lib().mpk_gemm_grouped_wgrad(_addr(A), lda, _addr(dD), ldg, ab_type, _addr(dB), d_type, ldd,
                                         _addr(offsets), E, M, N, K, s))
@@ -568,6 +582,8 @@ def _matrix(t, what: str, dim: int, dtype, like=None):
     if (len(shape) != dim or (dtype is not None and t.dtype is not dtype) or not t.is_cuda
             or (like is not None and t.get_device() != like.get_device())):
         _want(t, what, dim, dtype, None, like)
+    if max(shape) > 0x7FFFFFFF:
+        _sizes(*shape)
     return shape
 
 

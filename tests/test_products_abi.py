@@ -163,3 +163,35 @@ def test_allocating_forms_check_their_tensors(mpk_lib):
                 torch.zeros((1, 8)).expand(4, 8), torch.zeros((4, 16))[:, ::2]):
         with pytest.raises(ValueError):
             m._row_stride(bad, "x")
+
+
+def test_sizes_past_32_bits_are_refused(mpk_lib):
+    """Sizes that a C int cannot hold raise; 2^32 + 5 rows are not taken for 5."""
+    from types import SimpleNamespace
+
+    import torch
+
+    m = mpk_lib
+    big = (1 << 32) + 5
+    for sizes in ((big, 1, 1, 1), (1, big, 1, 1), (1, 1, big, 1), (1, 1, 1, big), (1, 1, 1, -big), (1, 1 << 31, 1, 1)):
+        E, M, N, K = sizes
+        for call in (lambda: m.gemm_grouped_gpu(PTR, K, PTR, N, m.B_KN, m.TYPE_BF16, PTR, m.TYPE_BF16, N, PTR, *sizes),
+                     lambda: m.gemm_grouped_wgrad_gpu(PTR, K, PTR, N, m.TYPE_BF16, PTR, m.TYPE_BF16, N, PTR, *sizes),
+                     lambda: m.gemm_grouped_int8_gpu(PTR, K, PTR, PTR, N, m.B_KN, PTR, PTR, m.TYPE_BF16, N, PTR,
+                                                     *sizes),
+                     lambda: m.gemm_grouped_mxfp8_gpu(PTR, PTR, PTR, N, PTR, PTR, PTR, *sizes)):
+            with pytest.raises(ValueError, match="32-bit"):
+                call()
+    for M, N, K in ((big, 1, 1), (1, big, 1), (1, 1, big)):
+        with pytest.raises(ValueError, match="32-bit"):
+            m.gemm_int8_gpu(PTR, K, PTR, PTR, N, m.B_KN, PTR, None, PTR, m.TYPE_BF16, N, M, N, K)
+        with pytest.raises(ValueError, match="32-bit"):
+            m.int8_quantize_cols_gpu(PTR, m.TYPE_BF16, K, PTR, K, PTR, M, N, K)
+        with pytest.raises(ValueError, match="32-bit"):
+            m.linear_int8_gpu(PTR, m.TYPE_BF16, K, PTR, N, m.B_KN, PTR, None, PTR, m.TYPE_BF16, N, M, N, K)
+    with pytest.raises(ValueError, match="32-bit"):
+        m.int8_quantize_rows_gpu(PTR, m.TYPE_BF16, 1, PTR, 1, PTR, big, 1)
+    # the allocating forms look at their tensors' shapes
+    t = SimpleNamespace(shape=(big, 1), dtype=torch.int8, is_cuda=True, get_device=lambda: 0)
+    with pytest.raises(ValueError, match="32-bit"):
+        m._matrix(t, "x", 2, torch.int8)
