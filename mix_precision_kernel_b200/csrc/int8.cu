@@ -216,16 +216,18 @@ int8_quantize_shifted_rows_kernel(const typename D::T* x, int64_t ldx, int8_t* c
 // rows, the strip's largest magnitudes are joined through distributed shared memory, and
 // a second pass over the share makes the codes.  The second pass finds the share in L2 on
 // the block's own side of the chip; two kernels with the maxima in memory between them,
-// or a share held in registers, took as long or longer (4096 x 12288 BF16: 37 us, 4.1
-// TB/s of the least bytes; 44 and 52 us).
+// or a share held in registers or shared memory, took as long or longer (4096 x 12288
+// BF16: 37 us, 4.1 TB/s of the least bytes; 44, 52 and 38 us).
 constexpr int kColThreads = 256;
-constexpr int kColBatch = 8;   // rows a thread has in flight
-constexpr int kColBlocks = 3;  // resident blocks per SM
+constexpr int kColBatch = 8;    // rows a thread has in flight
+constexpr int kColBlocks = 3;   // resident blocks per SM
+constexpr int kColWide = 16;    // threads across a strip
+constexpr int kColCtas = 8;     // most blocks per strip
+constexpr int kColShare = 512;  // rows of one of them, where there are strips enough
 
-template <class D, bool kVector>
+template <class D, bool kVector, int kAcross>  // kAcross threads across a strip
 struct Cols {
     static constexpr int V = kVector ? D::kVec : 1;
-    static constexpr int kAcross = 16;  // threads across a strip
     static constexpr int kStrip = kAcross * V;
     static constexpr int kDown = kColThreads / kAcross;  // rows per step
     using Piece = std::conditional_t<kVector, uint4, typename D::T>;
@@ -246,12 +248,12 @@ struct Cols {
     }
 };
 
-template <class D, bool kVector>
+template <class D, bool kVector, int kAcross>
 __global__ void __launch_bounds__(kColThreads, kColBlocks)
 int8_quantize_cols_kernel(const typename D::T* __restrict__ w, int64_t ldw, int8_t* __restrict__ codes,
                           int64_t ld_codes, float* __restrict__ scales, int64_t K, int64_t N)
 {
-    using S = Cols<D, kVector>;
+    using S = Cols<D, kVector, kAcross>;
     constexpr int V = S::V;
     constexpr bool kPacked = V == 8;  // two 16-bit magnitudes compared at once
     constexpr int kMax = kPacked ? 4 : V;
@@ -259,7 +261,7 @@ int8_quantize_cols_kernel(const typename D::T* __restrict__ w, int64_t ldw, int8
     __shared__ float sinv[S::kStrip];
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int tid = threadIdx.x, tx = tid % S::kAcross, ty = tid / S::kAcross;
+    const int tid = threadIdx.x, tx = tid % kAcross, ty = tid / kAcross;
     const int64_t e = blockIdx.y;
     const int64_t n0 = (int64_t)(blockIdx.x / ctas) * S::kStrip, n = n0 + tx * V;
     const int64_t share = (K + ctas - 1) / ctas;
@@ -379,18 +381,31 @@ cudaError_t cols(const void* w, int64_t ldw, int8_t* codes, int64_t ld_codes, fl
     const auto* in = static_cast<const typename D::T*>(w);
     const bool vec = N % D::kVec == 0 && aligned(w, ldw * (int64_t)sizeof(typename D::T), 16) &&
                      aligned(codes, ld_codes, D::kVec);
-    const int64_t strip = vec ? Cols<D, true>::kStrip : Cols<D, false>::kStrip;
-    const auto kernel = vec ? int8_quantize_cols_kernel<D, true> : int8_quantize_cols_kernel<D, false>;
-    constexpr unsigned kCtas = 8;
+    const int64_t sms = device_sm_count(), resident = kColBlocks * sms;
+    int64_t strip = kColWide * (vec ? D::kVec : 1);
+    // Blocks per strip: one for kColShare rows, more while SMs are without one (16 x 1024 x 4096
+    // BF16: 46 us with 2, 62 with 8; 32 x 256 x 2048: 15 with 1, 53 with 8; 1 x 1024 x 4096: 6.8 with
+    // 8, 9.1 with 2), fewer where they would only begin a second round (8192 x 8192: 57 us with 4
+    // in one round, 61 with 8 in 1.15).
+    const auto blocks = [&](int64_t ctas) { return (N + strip - 1) / strip * E * ctas; };
+    int ctas = 1;
+    while (ctas < kColCtas && (K > kColShare * ctas || blocks(ctas) < sms)) ctas *= 2;
+    if (ctas > 1 && blocks(ctas) > resident && blocks(ctas) * 4 <= resident * 5) ctas /= 2;
+    // Strips half as wide where SMs are still without a block (4001 x 1000 FP16: 12.5 -> 11.1 us).
+    const bool narrow = vec && blocks(ctas) < sms;
+    if (narrow) strip /= 2;
+    const auto kernel = narrow ? int8_quantize_cols_kernel<D, true, kColWide / 2>
+                        : vec  ? int8_quantize_cols_kernel<D, true, kColWide>
+                               : int8_quantize_cols_kernel<D, false, kColWide>;
     constexpr int64_t kMaxGridY = 65535;
     for (int64_t e = 0; e < E; e += kMaxGridY) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)((N + strip - 1) / strip) * kCtas, (unsigned)std::min(kMaxGridY, E - e));
+        cfg.gridDim = dim3((unsigned)((N + strip - 1) / strip) * ctas, (unsigned)std::min(kMaxGridY, E - e));
         cfg.blockDim = dim3(kColThreads);
         cfg.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = kCtas;
+        attr[0].val.clusterDim.x = ctas;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;

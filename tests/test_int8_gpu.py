@@ -95,6 +95,21 @@ def test_cols(mpk_lib, cuda, dtype, kind, E, K, N, pad, shift):
         assert np.array_equal(codes.cpu().numpy(), want_c[0]) and _same(scales.cpu().numpy(), want_s[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,K,N", [(160, 40, 128), (160, 513, 128), (150, 1025, 128), (40, 2049, 512), (64, 2100, 100),
+                                   (1, 700, 320), (1, 8, 24), (300, 17, 5), (9, 1, 2048)])
+def test_cols_of_every_split(mpk_lib, cuda, dtype, E, K, N):
+    """Many strips and few: one to eight blocks share a strip's rows, some of them without a row."""
+    rng = np.random.default_rng(E * 5 + K + N)
+    x = _values(rng, (E, K, N), "normal")
+    x[::3, -1] = np.inf  # the last block's row alone spoils every column of some matrices
+    w = _tensor(x, dtype)
+    want_c, want_s = _codes_64(w.float().cpu().numpy(), 1)
+    codes, scales = mpk_lib.quantize_int8_cols(w)
+    assert np.array_equal(codes.cpu().numpy(), want_c)
+    assert _same(scales.cpu().numpy(), want_s)
+
+
 def test_quantizers_leave_the_padding_and_take_no_rows(mpk_lib, cuda):
     import torch
 
