@@ -790,15 +790,13 @@ static int run_product(ProductArgs a, cudaStream_t st)
     if (int rc = take_workspace(a_bytes + b_bytes, st, &ws)) return rc;
     cudaError_t e = cudaSuccess;
     if (copy_a) {
-        e = cudaMemcpy2DAsync(ws, (size_t)lda * eb, a.A, (size_t)a.lda * eb, (size_t)a.K * eb, (size_t)a.M,
-                              cudaMemcpyDeviceToDevice, st);
+        e = launch_pad_rows(a.A, a.lda, ws, lda, a.M, a.K, eb, st);
         a.A = ws;
         a.lda = lda;
     }
     if (copy_b && e == cudaSuccess) {
         void* b = static_cast<uint8_t*>(ws) + a_bytes;
-        e = cudaMemcpy2DAsync(b, (size_t)ldb * eb, a.B, (size_t)a.ldb * eb, (size_t)b_cols * eb, (size_t)b_rows,
-                              cudaMemcpyDeviceToDevice, st);
+        e = launch_pad_rows(a.B, a.ldb, b, ldb, b_rows, b_cols, eb, st);
         a.B = b;
         a.ldb = ldb;
     }

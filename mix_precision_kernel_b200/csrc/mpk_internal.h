@@ -139,6 +139,10 @@ constexpr int kMaxGroups = 1024;
 // alignment; elements between K and the next multiple of 8 become zeros.
 cudaError_t launch_mxfp8_unpack_rows(const uint8_t* data, const uint8_t* scales, void* out, int64_t M, int64_t K,
                                      int64_t ld_out, cudaStream_t stream);
+// rows x cols elements of 1 or 2 bytes, rows ldx apart, to rows ld_out apart (a multiple of 16
+// bytes; out 16-byte aligned).  What follows a row's last element in its last 16 bytes is zero.
+cudaError_t launch_pad_rows(const void* x, int64_t ldx, void* out, int64_t ld_out, int64_t rows, int64_t cols,
+                            int elem_bytes, cudaStream_t stream);
 // Operands TMA can read in place: base and row strides multiples of 16 bytes.
 bool product_tma_ok(const void* p, int64_t ld, int elem_bytes);
 // Whether launch_product can quantize M rows of K itself (ProductArgs::x).

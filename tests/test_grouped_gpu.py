@@ -563,3 +563,34 @@ def test_overlapping_groups_stay_inside(mpk_lib, cuda, M, E, K):
     want = A[:M].double().t() @ A[:M, :128].double()
     _equal(dB[0], want, torch.float32)
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("K", [1, 7, 16, 33, 100, 515, 4099])
+def test_operands_at_every_address(mpk_lib, cuda, K):
+    """Bases and rows of A and B at all 16 places within 16 bytes, NaN all around 16-bit ones."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    M, N, E = 21, 40, 2
+    off = torch.tensor([0, 9, M], dtype=torch.int32, device="cuda")
+
+    def at(values, shift, fill):
+        shape, pad = values.shape, 1 + shift % 3
+        flat = torch.full((values.numel() // K * (K + pad) + 32,), fill, dtype=values.dtype, device="cuda")
+        view = flat[shift:shift + values.numel() // K * (K + pad)].view(*shape[:-1], K + pad)[..., :K]
+        view.copy_(values)
+        return view
+
+    a = torch.randint(-4, 5, (M, K), generator=gen, device="cuda")
+    b = torch.randint(-4, 5, (E, N, K), generator=gen, device="cuda")
+    want = torch.cat([a[:9].double() @ b[0].double().t(), a[9:].double() @ b[1].double().t()])
+    one, ones = torch.ones(M, device="cuda"), torch.ones((E, N), device="cuda")
+    for shift in range(16):
+        # sums of at most 16 * 4099 < 2^24 are exact in FP32
+        got = mpk_lib.gemm_grouped_int8(at(a.to(torch.int8), shift, 77), one, at(b.to(torch.int8), 15 - shift, 77),
+                                        ones, off, out_dtype=torch.float32, b_layout=mpk_lib.B_NK)
+        assert torch.equal(got.double(), want)
+        nan = float("nan")
+        got = mpk_lib.gemm_grouped(at(a.bfloat16(), shift % 8, nan), at(b.bfloat16(), (shift + 3) % 8, nan), off,
+                                   out_dtype=torch.float32, b_layout=mpk_lib.B_NK)
+        assert torch.equal(got.double(), want)
