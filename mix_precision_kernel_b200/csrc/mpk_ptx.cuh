@@ -188,6 +188,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// The same wait by a converged warp, with one answer for all its lanes.  Each lane tests
+// the barrier, the clock and the abort flag for itself, and where another warp gives up
+// just as the phase completes they may differ: lanes that went on alone would enter
+// warp-collective instructions (tcgen05.ld, shuffles) that the others never reach.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                               int* status, int site, uint64_t timeout_ns)
+{
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, site, timeout_ns));
+}
+
 // ---------------------------------------------------------------------------
 // TMA (tensor copies global -> shared, completion through an mbarrier)
 // ---------------------------------------------------------------------------

@@ -325,6 +325,7 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
     const int nvec = p.x_vec ? p.K / V : 0;
     const int start = (ew % warps) * 32 + lane, stride = warps * 32;
     if (ew == 0 && lane < kFusedRows) amax_bits[lane] = 0u;
+    __syncwarp();
     named_bar_sync(1, 32 * kFuseWarps);
     for (int m = ew / warps; m < M; m += kFuseWarps / warps) {
         const typename T::T* row = static_cast<const typename T::T*>(p.x) + m * p.ldx;
@@ -340,6 +341,7 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
         a = __reduce_max_sync(0xFFFFFFFFu, a);
         if (lane == 0) atomicMax(&amax_bits[m], a);  // a maximum has no order
     }
+    __syncwarp();
     named_bar_sync(1, 32 * kFuseWarps);
     for (int m = ew / warps; m < M; m += kFuseWarps / warps) {
         const typename T::T* row = static_cast<const typename T::T*>(p.x) + m * p.ldx;
@@ -363,6 +365,7 @@ __device__ __forceinline__ void make_codes(const Params& p, int ew, int lane, in
             *at(k) = rs.inv == 0.0f ? (uint8_t)0 : (uint8_t)int8::code_bits(T::widen(row[k]), rs.inv);
     }
     fence_proxy_async_smem();
+    __syncwarp();
     named_bar_sync(1, 32 * kFuseWarps);
 }
 
@@ -799,8 +802,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
             const int last = (s + k1 - k0 - 1) % S;
             s = (last + 1) % S;
             if (rows == 0) continue;
-            ok = mbar_wait(tail(last), (phases >> last) & 1u, abort_flag, p.status, kSiteTail, p.timeout_ns);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            ok = mbar_wait_warp(tail(last), (phases >> last) & 1u, abort_flag, p.status, kSiteTail, p.timeout_ns);
             if (!ok) break;
             phases ^= 1u << last;
             const int end = (rows + 15) / 16 * 16;
@@ -861,7 +863,8 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                     sa[j] = r < x.rows ? (C::kFuse ? fused_scales[r & (kFusedRows - 1)] : p.a_scales[row0 + r]) : 0.0f;
                 }
             }
-            if (!mbar_wait(tfull(acc), (uint32_t)(it >> 1) & 1u, abort_flag, p.status, kSiteTmemFull, p.timeout_ns))
+            if (!mbar_wait_warp(tfull(acc), (uint32_t)(it >> 1) & 1u, abort_flag, p.status, kSiteTmemFull,
+                                p.timeout_ns))
                 break;
             tc_fence_after();
             const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * p.acc_cols);
@@ -869,6 +872,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                 int j = 0;
 #pragma unroll 1
                 for (int c = 32 * turn; c < x.rows; c += 32 * C::kTurns, ++j) {
+                    __syncwarp();  // lanes past N leave a chunk's stores early; the load takes the whole warp
                     uint32_t raw[32];
                     if (any) {
                         tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
@@ -934,16 +938,17 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                 const int r = ew * 32 + lane;
                 if (r < x.rows) tile_scales[r] = C::kFuse ? fused_scales[r & (kFusedRows - 1)] : p.a_scales[row0 + r];
             }
-            ok = mbar_wait(tfull(0), 0, abort_flag, p.status, kSiteTmemFull, p.timeout_ns);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            ok = mbar_wait_warp(tfull(0), 0, abort_flag, p.status, kSiteTmemFull, p.timeout_ns);
             tc_fence_after();
         }
+        __syncwarp();  // columns past N loaded no scales; the barriers take whole warps
         if (p.parts_in_ring) cluster_sync_all();
         if (busy && ok) {
             const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16);
             const uint32_t mine = smem_u32(parts) + 16u * (uint32_t)(split * share * kCols + quad * 32 + lane);
 #pragma unroll 1
             for (int c = 32 * turn; c < x.rows; c += 32 * C::kTurns) {
+                __syncwarp();
                 uint32_t raw[32];
                 if (k1 > k0) {
                     tmem_ld_32x32b_x32(tacc + (uint32_t)c, raw);
@@ -963,6 +968,7 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                 }
             }
         }
+        __syncwarp();
         cluster_sync_all();
         if (busy && *abort_flag == 0) {
             const uint4* part = reinterpret_cast<const uint4*>(parts) + quad * 32 + lane;

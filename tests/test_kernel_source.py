@@ -1,0 +1,60 @@
+"""Rules of the kernels' source that no run can show: what they prevent needs a wait to
+give up at one moment in one warp, and then hangs the GPU (no GPU needed)."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mix_precision_kernel_b200", "csrc")
+
+
+def _source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        text = f.read()
+    return re.sub(r"//[^\n]*", "", text)  # comments name the functions too
+
+
+def _block(text, start):
+    """The brace-enclosed block that opens at or after `start`."""
+    at = text.index("{", start)
+    depth = 0
+    for i in range(at, len(text)):
+        depth += (text[i] == "{") - (text[i] == "}")
+        if depth == 0:
+            return text[at:i + 1]
+    raise AssertionError("unbalanced braces")
+
+
+def test_warps_leave_a_wait_together():
+    """Lanes of a warp see a wait expire each for itself, so a whole warp that waits takes a
+    vote before it branches.  Only the elected lane of a producer or issuer waits alone."""
+    text = _source("products.cu")
+    kernel = _block(text, text.index("product_kernel(const __grid_constant__"))
+    alone = []
+    for elected in re.finditer(r"if \((?:rank == 0 && )?elect_one\(\)\) ", kernel):
+        alone.append(_block(kernel, elected.end()))
+    assert len(alone) == 2 and all("mbar_wait(" in a for a in alone)
+    together = kernel
+    for a in alone:
+        together = together.replace(a, "")
+    assert "mbar_wait(" not in together
+    # the tail rows, the epilogue of whole tiles and the join of split ones
+    assert together.count("mbar_wait_warp(") == 3
+    helper = _block(_source("mpk_ptx.cuh"), _source("mpk_ptx.cuh").index("bool mbar_wait_warp("))
+    assert re.search(r"__all_sync\(0xFFFFFFFFu, mbar_wait\(", helper)
+
+
+def test_warps_meet_before_warp_wide_instructions():
+    """Lanes past N leave a chunk's stores early, and rows of x end in different lanes: the
+    aligned instructions that follow come after a __syncwarp."""
+    text = _source("products.cu")
+    kernel = _block(text, text.index("product_kernel(const __grid_constant__"))
+    chunks = [_block(kernel, m.end()) for m in re.finditer(r"for \(int c = 32 \* turn; [^{]*", kernel)]
+    assert len(chunks) == 2
+    for c in chunks:
+        assert 0 < c.index("__syncwarp()") < c.index("tmem_ld_32x32b_x32(")
+    for scope in (_block(kernel, kernel.index("if (p.splits > 1 && unit")),
+                  _block(text, text.index("void make_codes("))):
+        syncs = list(re.finditer(r"(?:cluster_sync_all|named_bar_sync)\(", scope))
+        assert syncs
+        for s in syncs:
+            before = re.split(r"[;{}]", scope[:s.start()])
+            assert "__syncwarp()" in before[-2], scope[s.start() - 120:s.end()]
