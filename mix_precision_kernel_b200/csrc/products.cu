@@ -41,7 +41,8 @@
 // stores (weight gradient of 32 x 2048x2816 BF16 in 87 us, 4.2 TB/s).
 //
 // Every mbarrier wait is bounded (mpk::mbar_wait); on expiry the CTA raises an abort
-// flag, records a status code, drains what it has in flight and leaves.
+// flag (where a cluster joins its sums, that of all its CTAs), records a status code, drains
+// what it has in flight and leaves.  What it has not stored by then stays as it was.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -939,6 +940,10 @@ product_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant
                 if (r < x.rows) tile_scales[r] = C::kFuse ? fused_scales[r & (kFusedRows - 1)] : p.a_scales[row0 + r];
             }
             ok = mbar_wait_warp(tfull(0), 0, abort_flag, p.status, kSiteTmemFull, p.timeout_ns);
+            // A part that never came must not be added: the whole cluster stores nothing.  The
+            // barrier below makes the flags visible before any CTA looks at its own.
+            if (!ok && lane < ctas)
+                st_shared_cluster_u32(mapa_shared(smem_u32(const_cast<int*>(abort_flag)), (uint32_t)lane), 1u);
             tc_fence_after();
         }
         __syncwarp();  // columns past N loaded no scales; the barriers take whole warps

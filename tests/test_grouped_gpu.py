@@ -594,3 +594,32 @@ def test_operands_at_every_address(mpk_lib, cuda, K):
         got = mpk_lib.gemm_grouped(at(a.bfloat16(), shift % 8, nan), at(b.bfloat16(), (shift + 3) % 8, nan), off,
                                    out_dtype=torch.float32, b_layout=mpk_lib.B_NK)
         assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("M,K,N", [(4000000, 64, 64), (1000000, 2048, 2048)], ids=["cluster", "pairs"])
+def test_a_wait_that_runs_out_is_reported(mpk_lib, cuda, M, K, N):
+    """Reductions of milliseconds under a wait budget of a microsecond: the epilogue's waits give
+    up (a wait parks for up to a millisecond per test, and tests twice), in a cluster that
+    shares one tile's reduction and in pairs with a tile each.  The call returns, nothing of D is
+    written, the status word says so, and the next call with the usual budget is right."""
+    import torch
+
+    m = mpk_lib
+    A = torch.ones((M, K), dtype=torch.bfloat16, device="cuda")
+    G = torch.ones((M, N), dtype=torch.bfloat16, device="cuda")
+    G[M // 2:] = -1.0
+    off = _offsets([M])
+    dB = torch.full((1, K, N), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    m.set_wait_timeout_ns(1000)
+    try:
+        m.gemm_grouped_wgrad(A, G, off, out=dB)
+        torch.cuda.synchronize()
+    finally:
+        m.set_wait_timeout_ns(2_000_000_000)
+    assert m.device_status() == 0x124
+    assert bool((dB == 7).all())
+    m.gemm_grouped_wgrad(A, G, off, out=dB)
+    assert m.device_status() == 0
+    # M / 2 ones and M / 2 minus ones: whole numbers below 2^24
+    assert bool((dB == 0).all())

@@ -58,3 +58,20 @@ def test_warps_meet_before_warp_wide_instructions():
         for s in syncs:
             before = re.split(r"[;{}]", scope[:s.start()])
             assert "__syncwarp()" in before[-2], scope[s.start() - 120:s.end()]
+
+
+def test_an_expired_wait_stops_the_whole_join():
+    """CTAs that share a tile's reduction hand their sums to one another.  One whose wait gave up
+    hands over nothing: it raises the flag of every CTA of the cluster before the barrier
+    behind which the sums are added, and each looks at its flag there."""
+    text = _source("products.cu")
+    kernel = _block(text, text.index("product_kernel(const __grid_constant__"))
+    join = _block(kernel, kernel.index("if (p.splits > 1 && unit"))
+    wait = join.index("mbar_wait_warp(")
+    raised = re.search(r"if \(!ok && lane < ctas\)\s*st_shared_cluster_u32\(mapa_shared\("
+                       r"smem_u32\(const_cast<int\*>\(abort_flag\)\), \(uint32_t\)lane\), 1u\);", join)
+    assert raised and wait < raised.start()
+    parts = join.index("st_shared_cluster_v4(")
+    barrier = join.index("cluster_sync_all();", parts)
+    added = join.index("if (busy && *abort_flag == 0)")
+    assert raised.end() < parts < barrier < added
