@@ -769,7 +769,7 @@ __device__ __forceinline__ void run_epilogue(const Params& p, uint32_t tmem_base
         const int nchunks = min(bn / 32, (p.N - n0 + 31) / 32);
         if (kStreamK && u.kind == kUnitContrib) {
             const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
-            if (!mbar_wait(tfull(acc), acc_ph, abort_flag, p.status, kSiteTmemFull, p.timeout_ns)) break;
+            if (!mbar_wait_warp(tfull(acc), acc_ph, abort_flag, p.status, kSiteTmemFull, p.timeout_ns)) break;
             tc_fence_after();
             sk_store_partial(sk_slot(p, cluster, rank) + r, tacc, row_ok, nchunks);
             tc_fence_before();
@@ -807,7 +807,7 @@ __device__ __forceinline__ void run_epilogue(const Params& p, uint32_t tmem_base
                 }
             }
             if (!full_seen) {
-                if (!mbar_wait(tfull(acc), acc_ph, abort_flag, p.status, kSiteTmemFull, p.timeout_ns)) {
+                if (!mbar_wait_warp(tfull(acc), acc_ph, abort_flag, p.status, kSiteTmemFull, p.timeout_ns)) {
                     aborted = true;
                     break;
                 }
@@ -850,7 +850,7 @@ __device__ __forceinline__ void run_epilogue(const Params& p, uint32_t tmem_base
         if (aborted) break;
         // An item with no columns inside N (the second half of a split tile at the
         // right edge) still waits for its accumulator phase, so that phases pair up.
-        if (!full_seen && !mbar_wait(tfull(acc), acc_ph, abort_flag, p.status, kSiteTmemFull, p.timeout_ns))
+        if (!full_seen && !mbar_wait_warp(tfull(acc), acc_ph, abort_flag, p.status, kSiteTmemFull, p.timeout_ns))
             break;
         tc_fence_before();
         __syncwarp();
@@ -915,7 +915,7 @@ __device__ __forceinline__ void run_epilogue_onchip(const Params& p, uint32_t tm
                 }
             }
         }
-        if (!mbar_wait(tfull, (uint32_t)it & 1u, abort_flag, p.status, kSiteTmemFull, p.timeout_ns)) break;
+        if (!mbar_wait_warp(tfull, (uint32_t)it & 1u, abort_flag, p.status, kSiteTmemFull, p.timeout_ns)) break;
         tc_fence_after();
         const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16);
         if (p.vec_cd && n0 + BN <= p.N) {
@@ -1224,8 +1224,8 @@ gemm_mxfp8_bf16_kernel(const __grid_constant__ CUtensorMap tmap_a,
                     // Waiting on it first also keeps every group within STAGES (<=
                     // A8_STAGES) stages of the MMA, so no parity wait below can match a
                     // phase one round too old.
-                    if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, p.status, kSiteEmptyT, p.timeout_ns) ||
-                        !mbar_wait(a8_full(j8), ph8, abort_flag, p.status, kSiteFullA8, p.timeout_ns)) {
+                    if (!mbar_wait_warp(empty(s), ph ^ 1u, abort_flag, p.status, kSiteEmptyT, p.timeout_ns) ||
+                        !mbar_wait_warp(a8_full(j8), ph8, abort_flag, p.status, kSiteFullA8, p.timeout_ns)) {
                         ok = false;
                         break;
                     }

@@ -75,3 +75,23 @@ def test_an_expired_wait_stops_the_whole_join():
     barrier = join.index("cluster_sync_all();", parts)
     added = join.index("if (busy && *abort_flag == 0)")
     assert raised.end() < parts < barrier < added
+
+
+def test_warps_of_the_gemm_kernels_leave_a_wait_together():
+    """The same rule in the MXFP8 GEMM: epilogues and the on-chip kernel's transform wait as warps."""
+    text = _source("gemm.cu")
+    alone = 0
+    for name in ("void run_epilogue(", "void run_epilogue_onchip("):
+        body = _block(text, text.index("\n{", text.index(name)))  # behind a default argument's braces
+        for single in re.finditer(r"if \(lane == 0\) (?=\{)", body):
+            block = _block(body, single.end())
+            alone += block.count("mbar_wait(")
+            body = body.replace(block, "")
+        assert "mbar_wait(" not in body and "mbar_wait_warp(" in body
+        # adding partials waits lane by lane, and its callers vote
+        for call in re.finditer(r"const bool ok = sk_add_pieces\([^;]*;\s*", body):
+            assert body[call.end():].startswith("if (!__all_sync(0xFFFFFFFFu, ok))")
+    assert alone == 1
+    transform = _block(text, text.index("} else if (warp < kFirstEpilogueWarp) ") + 1)
+    assert "tmem_st_32x32b_x16(" in transform
+    assert "mbar_wait(" not in transform and transform.count("mbar_wait_warp(") == 2
