@@ -225,13 +225,15 @@ int mpk_int8_quantize_cols(const void* w, int w_type, int64_t ldw, int8_t* codes
  * (FP32 [N], may be NULL) is added, and the result is rounded once to D's type.
  * b_layout: MPK_B_KN or MPK_B_NK.  lda, ldb, ldd: row strides in elements.  Any size
  * and alignment; operands whose base or row stride is not a multiple of 16 bytes are
- * first copied into a workspace of the library's pool.  No counterpart in the reference. */
+ * first copied into a workspace of the library's pool.  D must not overlap the operands.
+ * No counterpart in the reference. */
 int mpk_gemm_int8(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb, int b_layout,
                   const float* B_scales, const float* bias, void* D, int d_type, int64_t ldd, int M, int N, int K,
                   void* stream);
 
 /* mpk_int8_quantize_rows of x, then mpk_gemm_int8: a linear layer with int8 weights and
- * activations quantized per token.  The codes live in a workspace of the library's pool. */
+ * activations quantized per token.  The codes live in a workspace of the library's pool.  D
+ * may lie in x's place; it must not overlap the other operands. */
 int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int64_t ldb, int b_layout,
                     const float* B_scales, const float* bias, void* D, int d_type, int64_t ldd, int M, int N, int K,
                     void* stream);

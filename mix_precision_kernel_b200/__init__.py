@@ -699,7 +699,7 @@ def gemm_int8(A, A_scales, B, B_scales, bias=None, out_dtype=None, b_layout: int
 
 def linear_int8(x, B, B_scales, bias=None, out_dtype=None, b_layout: int = B_KN, out=None):
     """gemm_int8 of x [M, K] (float32, bfloat16 or float16) quantized per row on the way; D in
-    out_dtype (default x's type)."""
+    out_dtype (default x's type).  out may lie in x's place."""
     torch = _torch or _init_torch()
     M, K = _matrix(x, "x", 2, None)
     t = _type_code(x.dtype, "x")

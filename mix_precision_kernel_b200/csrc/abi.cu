@@ -651,6 +651,15 @@ static int check_matrix(const char* what, int64_t count, int64_t rows, int64_t c
     return MPK_SUCCESS;
 }
 
+// Whether the addresses from the first to the last element of two matrices have any in common.
+static bool ranges_meet(const void* p, int64_t p_rows, int64_t p_cols, int64_t p_ld, int p_bytes, const void* q,
+                        int64_t q_rows, int64_t q_cols, int64_t q_ld, int q_bytes)
+{
+    const uintptr_t p0 = reinterpret_cast<uintptr_t>(p), q0 = reinterpret_cast<uintptr_t>(q);
+    return p0 < q0 + (uintptr_t)(((q_rows - 1) * q_ld + q_cols) * q_bytes) &&
+           q0 < p0 + (uintptr_t)(((p_rows - 1) * p_ld + p_cols) * p_bytes);
+}
+
 static int check_aligned(const void* x, int bytes, const float* scales)
 {
     if (reinterpret_cast<uintptr_t>(x) % bytes || reinterpret_cast<uintptr_t>(scales) % 4) {
@@ -891,7 +900,9 @@ int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int
     if (int rc = check_matrix("x", 1, M, K, ldx, type_bytes(x_type))) return rc;
     if (int rc = check_aligned(x, type_bytes(x_type), nullptr)) return rc;
     if (int rc = check_arch()) return rc;
-    if (product_quantizes(M, K)) {
+    // Where every CTA quantizes x for itself, none may overwrite it with its columns of D while
+    // another still reads it: a D in x's place takes the quantizer in front.
+    if (product_quantizes(M, K) && !ranges_meet(x, M, K, ldx, type_bytes(x_type), D, M, N, ldd, type_bytes(d_type))) {
         a.x = x, a.ldx = ldx, a.x_type = x_type;
         return run_product(a, st);
     }

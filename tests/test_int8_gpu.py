@@ -361,3 +361,24 @@ def test_fused_and_separate_quantizers_agree(mpk_lib, cuda):
             assert torch.equal(got.nan_to_num(7.0), all_rows[:n].nan_to_num(7.0))
             assert torch.equal(got.isnan(), all_rows[:n].isnan())
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K", [(1, 4096), (1, 8192), (2, 4096), (16, 512), (7, 500), (17, 1024), (300, 264)])
+def test_linear_in_place_of_its_input(mpk_lib, cuda, dtype, M, K):
+    """D written over x, or a row further down in x's tensor, is the D of a call that keeps x,
+    for rows that the product quantizes itself as for more."""
+    import torch
+
+    m = mpk_lib
+    rng = np.random.default_rng(M + K)
+    x = _tensor(_values(rng, (M, K), "normal"), dtype)
+    B, sb = m.quantize_int8_cols(_tensor(_values(rng, (K, K), "normal"), "float32"))
+    want = m.linear_int8(x, B, sb)
+    for down in (0, 1):
+        for _ in range(5):
+            whole = torch.zeros((M + 1, K), dtype=x.dtype, device="cuda")
+            whole[:M] = x
+            m.linear_int8(whole[:M], B, sb, out=whole[down:M + down])
+            assert torch.equal(whole[down:M + down], want)
+    assert m.device_status() == 0
