@@ -623,3 +623,41 @@ def test_a_wait_that_runs_out_is_reported(mpk_lib, cuda, M, K, N):
     assert m.device_status() == 0
     # M / 2 ones and M / 2 minus ones: whole numbers below 2^24
     assert bool((dB == 0).all())
+
+
+# Groups whose tiles are shared by pairs of CTAs (more than 48 rows per group, enough tiles),
+# with more tiles than pairs and, in the longest group, more than one panel of row tiles.
+MANY = [4500, 3, 700]
+
+
+@pytest.mark.parametrize("poisoned", [None, 0, 1, 2])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("N,K", [(1304, 200), (1003, 131)])
+def test_many_tiles_are_exact(mpk_lib, cuda, dtype, layout, poisoned, N, K):
+    """The kernels of long batches, with a group whose rows and weights are not finite beside
+    groups that must not see them, and rows in front of and behind all groups."""
+    import torch
+
+    m = mpk_lib
+    t = getattr(torch, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    first, behind = 5, 9
+    M, E = first + sum(MANY) + behind, len(MANY)
+    for out, pad in ((t, 8), (torch.float32, 3)):
+        A = _ints((M, K), gen, t, pad)
+        B = _ints((E, K, N) if layout == "kn" else (E, N, K), gen, t, pad)
+        A[:first], A[M - behind:] = float("inf"), float("nan")
+        if poisoned is not None:
+            lo = first + sum(MANY[:poisoned])
+            A[lo:lo + MANY[poisoned]] = float("nan")
+            B[poisoned] = float("inf")
+        whole = torch.full((M, N + 8), 5.0, dtype=out, device="cuda")
+        D = m.gemm_grouped(A, B, _offsets(MANY, first), b_layout=m.B_KN if layout == "kn" else m.B_NK,
+                           out=whole[:, :N])
+        want = _product_64(A, B if layout == "kn" else B.transpose(1, 2), MANY, first)
+        want[:first] = 5.0
+        want[M - behind:] = 5.0
+        _equal(D, want, out)
+        assert bool((whole[:, N:] == 5).all())
+    assert m.device_status() == 0

@@ -382,3 +382,56 @@ def test_linear_in_place_of_its_input(mpk_lib, cuda, dtype, M, K):
             m.linear_int8(whole[:M], B, sb, out=whole[down:M + down])
             assert torch.equal(whole[down:M + down], want)
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("M,N,K", [(1030, 2570, 200), (2100, 2570, 200), (4500, 1300, 130), (40, 19500, 64)])
+def test_product_of_many_tiles(mpk_lib, cuda, M, N, K, layout):
+    """Sizes at which pairs of CTAs share a tile (the first three), a CTA has more tiles than one,
+    so that its second accumulator and both accumulators' row scales come into use (the
+    last three), and a row's tiles make more than one panel (4500 rows)."""
+    import torch
+
+    m = mpk_lib
+    gen = torch.Generator(device="cuda").manual_seed(M + N + K)
+    a = torch.randint(-128, 128, (M, K), generator=gen, device="cuda").to(torch.int8)
+    b = torch.randint(-128, 128, (K, N), generator=gen, device="cuda").to(torch.int8)
+    sa = (torch.rand(M, generator=gen, device="cuda") + 0.5) * 2.0 ** -10
+    sb = (torch.rand(N, generator=gen, device="cuda") + 0.5) * 2.0 ** -8
+    sa[3 % M], sa[M - 1], sb[N - 2] = float("nan"), float("inf"), float("nan")
+    bias = torch.randn(N, generator=gen, device="cuda")
+    acc = a.double() @ b.double()
+    want = acc.float() * sa[:, None] * sb
+    kept = b if layout == "kn" else b.t()
+    for pad, dtype, add in ((16 - kept.shape[1] % 16, torch.bfloat16, None), (16 - kept.shape[1] % 16, torch.float32, bias),
+                            (1, torch.float16, bias)):
+        B = torch.full((kept.shape[0], kept.shape[1] + pad), 77, dtype=torch.int8, device="cuda")[:, :kept.shape[1]]
+        B.copy_(kept)
+        A = torch.full((M, K + (-K) % 16 + 16), 77, dtype=torch.int8, device="cuda")[:, :K]
+        A.copy_(a)
+        whole = torch.full((M + 1, N + 6), 5.0, dtype=dtype, device="cuda")
+        D = m.gemm_int8(A, sa, B, sb, add, b_layout=m.B_KN if layout == "kn" else m.B_NK, out=whole[:M, :N])
+        full = (want if add is None else want + add).to(dtype)
+        assert bool(((D == full) | (D.isnan() & full.isnan())).all())
+        assert bool((whole[M:] == 5).all()) and bool((whole[:, N:] == 5).all())
+    assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 19500, 130), (1, 40000, 64), (16, 19500, 72), (3, 38000, 2048)])
+def test_fused_codes_serve_many_tiles(mpk_lib, cuda, dtype, M, N, K):
+    """More columns than the SMs take at once: a CTA multiplies the codes that it made with the
+    weights of its second and third tile too."""
+    import torch
+
+    m = mpk_lib
+    gen = torch.Generator(device="cuda").manual_seed(M + N + K)
+    x = torch.randn((M, K), generator=gen, device="cuda").to(getattr(torch, dtype))
+    x[M - 1, K // 2] = float("nan") if M > 1 else 9.0
+    B = torch.randint(-127, 128, (K, N), generator=gen, device="cuda").to(torch.int8)
+    sb = torch.rand(N, generator=gen, device="cuda")
+    q, s = m.quantize_int8(x)
+    want = (q.double() @ B.double()).float() * s[:, None] * sb
+    D = m.linear_int8(x, B, sb, out_dtype=torch.float32)
+    assert bool(((D == want) | (D.isnan() & want.isnan())).all())
+    assert m.device_status() == 0
