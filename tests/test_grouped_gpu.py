@@ -661,3 +661,80 @@ def test_many_tiles_are_exact(mpk_lib, cuda, dtype, layout, poisoned, N, K):
         _equal(D, want, out)
         assert bool((whole[:, N:] == 5).all())
     assert m.device_status() == 0
+
+
+def _mx_values(rng, M, K):
+    """FP32 values that MXFP8 holds exactly: integers times a power of two per row."""
+    return rng.integers(-8, 9, (M, K)).astype(np.float32) * np.exp2(rng.integers(-2, 3, (M, 1))).astype(np.float32)
+
+
+def _check_mxfp8(D, Ds, exact64, rows):
+    """Codes and scales of `rows` against the oracle's quantization of the exact sums."""
+    import oracle as O
+
+    want, want_s = O.quantize(np.ascontiguousarray(exact64.float().cpu().numpy()[rows]))
+    got, got_s = D.cpu().numpy()[rows], Ds.cpu().numpy()[rows]
+    assert np.array_equal(got_s, want_s)
+    bad = (got != want) & ~((got & 0x7F == 0) & (want & 0x7F == 0))  # zeros carry no sign to speak of
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist())
+
+
+@pytest.mark.parametrize("sizes,K", [(MANY, 256), (MANY, 200), ([40], 2048), ([33, 0, 7], 2048), ([1], 4096),
+                                     ([300], 1024)], ids=str)
+@pytest.mark.parametrize("N", [1304, 1280, 77, 256])
+def test_mxfp8_of_every_kernel_with_nan_and_infinity(mpk_lib, cuda, sizes, K, N):
+    """Tiles of pairs, of single CTAs and of clusters that share a reduction make the same codes
+    and scales: NaN does not enter a block's largest magnitude and becomes the code 0x7F; an
+    infinity gives its block the scale 255, whose inverse is 0.  Both in rows of A (every
+    value of those rows of D) and in single weights (a column of D, beside finite ones)."""
+    import torch
+
+    import oracle as O
+
+    m = mpk_lib
+    rng = np.random.default_rng(K + N + len(sizes))
+    gen = torch.Generator(device="cuda").manual_seed(K + N)
+    M, E = sum(sizes), len(sizes)
+    values = _mx_values(rng, M, K)
+    codes, scales = O.quantize(values)
+    codes[M // 3, K // 2] = 0x7F  # NaN
+    scales[M // 2, K // 64] = 255  # 0 * inf and x * inf
+    values = O.dequantize(codes, scales)
+    B = _ints((E, K, N), gen, torch.bfloat16, pad=8)
+    B[0, K // 3, 5], B[0, 1, 40], B[0, 2, 41] = float("inf"), float("nan"), float("-inf")
+    D, Ds = m.gemm_grouped_mxfp8(torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda(), B, _offsets(sizes))
+    _check_mxfp8(D, Ds, _product_64(torch.from_numpy(values).cuda(), B, sizes), slice(0, M))
+    assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("shift", range(8))
+@pytest.mark.parametrize("K", [64, 96, 200, 33])
+def test_mxfp8_codes_at_every_address(mpk_lib, cuda, K, shift):
+    """Codes and scales anywhere, with the bytes around them holding NaN: whole blocks take the
+    codec's pre-pass where they are aligned and the product's own unpacking elsewhere.  Scale
+    bytes 0 (the value 0) and 255 (infinity) and NaN codes among them."""
+    import torch
+
+    import oracle as O
+
+    m = mpk_lib
+    rng = np.random.default_rng(K + shift)
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    sizes = [9, 0, 50]
+    M, N = sum(sizes), 72
+    values = _mx_values(rng, M, K)
+    codes, scales = O.quantize(values)
+    codes[4, K - 1], codes[20, 0] = 0x7F, 0xFF
+    scales[7, :], scales[30, -1] = 0, 255
+    values = O.dequantize(codes, scales)
+
+    def at(x):
+        flat = torch.full((x.size + 16,), 0xFF, dtype=torch.uint8, device="cuda")
+        view = flat[shift:shift + x.size].view(x.shape)
+        view.copy_(torch.from_numpy(x))
+        return view
+
+    B = _ints((3, K, N), gen, torch.bfloat16, pad=8)
+    D, Ds = m.gemm_grouped_mxfp8(at(codes), at(scales), B, _offsets(sizes))
+    _check_mxfp8(D, Ds, _product_64(torch.from_numpy(values).cuda(), B, sizes), slice(0, M))
+    assert m.device_status() == 0
