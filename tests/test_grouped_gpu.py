@@ -738,3 +738,53 @@ def test_mxfp8_codes_at_every_address(mpk_lib, cuda, K, shift):
     D, Ds = m.gemm_grouped_mxfp8(at(codes), at(scales), B, _offsets(sizes))
     _check_mxfp8(D, Ds, _product_64(torch.from_numpy(values).cuda(), B, sizes), slice(0, M))
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("K", [512, 500])
+def test_mxfp8_operands_written_just_before(mpk_lib, cuda, K):
+    """The grouped MXFP8 product reads its offsets and loads weights while its own unpacking kernel
+    runs.  Back to back on one stream: offsets, weights, codes and scales rewritten just in
+    front of it, then weights that the gradient's kernel (which lets its successor start early)
+    has just written; the codec's pre-pass (K = 512) and the product's unpacking (K = 500)."""
+    import torch
+
+    import oracle as O
+
+    m = mpk_lib
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    rng = np.random.default_rng(K)
+    E, M, N, rounds = 3, 600, 1024, 10
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    w = torch.empty((E, K, N), dtype=torch.bfloat16, device="cuda")
+    codes = torch.empty((M, K), dtype=torch.uint8, device="cuda")
+    scales = torch.empty((M, m.nblk(K)), dtype=torch.uint8, device="cuda")
+    values = [_mx_values(rng, M, K) for _ in range(rounds)]
+    quantized = [[torch.from_numpy(t).cuda() for t in O.quantize(v)] for v in values]
+    ws = [_ints((E, K, N), gen, torch.bfloat16) for _ in range(rounds)]
+    xs = [_ints((M, K), gen, torch.bfloat16, span=1) for _ in range(rounds)]
+    gs = [_ints((M, N), gen, torch.bfloat16, span=1) for _ in range(rounds)]
+    splits = [[0, 60 + 11 * i, 300 + 7 * i, M] for i in range(rounds)]
+    offs = [torch.tensor(s, dtype=torch.int32, device="cuda") for s in splits]
+    first = [(torch.empty((M, N), dtype=torch.uint8, device="cuda"),
+              torch.empty((M, m.nblk(N)), dtype=torch.uint8, device="cuda")) for _ in range(rounds)]
+    second = [tuple(torch.empty_like(t) for t in pair) for pair in first]
+    w_grad = []
+    torch.cuda.synchronize()
+    for i in range(rounds):
+        codes.copy_(quantized[i][0])
+        scales.copy_(quantized[i][1])
+        w.copy_(ws[i])
+        off.copy_(offs[i])
+        m.gemm_grouped_mxfp8(codes, scales, w, off, out=first[i])
+        m.gemm_grouped_wgrad(xs[i], gs[i], off, out=w)
+        m.gemm_grouped_mxfp8(codes, scales, w, off, out=second[i])
+        w_grad.append(w.clone())
+    torch.cuda.synchronize()
+    for i in range(rounds):
+        sizes = np.diff(splits[i]).tolist()
+        v = torch.from_numpy(values[i]).cuda()
+        _check_mxfp8(*first[i], _product_64(v, ws[i], sizes), slice(0, M))
+        _equal(w_grad[i], _wgrad_64(xs[i], gs[i], sizes), torch.bfloat16)
+        # |w| <= 390 and 512 terms of at most 32 * 390 in steps of 1/4: exact in FP32
+        _check_mxfp8(*second[i], _product_64(v, w_grad[i], sizes), slice(0, M))
+    assert m.device_status() == 0
