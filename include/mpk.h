@@ -51,7 +51,8 @@ enum {
  * src/kernels/gemm_fp8_tensorcore.cu:231-249).  Any M, N, K >= 0 and any pointer
  * alignment, as in the reference.  C_data/C_scales may both be NULL (no C term).
  *
- * A is dequantized exactly to BF16 by a bandwidth pre-pass into a workspace taken
+ * A is dequantized to BF16 (exactly for scale bytes 3 to 246, see
+ * mpk_gemm_grouped_mxfp8) by a bandwidth pre-pass into a workspace taken
  * from the library's pool on `stream` (rows padded to a multiple of 8 elements; B is
  * also copied there with padded rows when N % 8 != 0 or B is not 16-byte aligned),
  * then the tensor-core kernel streams both operands by TMA.  While `stream` is
@@ -247,12 +248,18 @@ int mpk_linear_int8(const void* x, int x_type, int64_t ldx, const int8_t* B, int
  * MPK_MAX_GROUPS.  Nothing is copied to the host: the calls can be captured.
  *
  * mpk_gemm_grouped: A and B of the same 16-bit type (MPK_TYPE_BF16 or MPK_TYPE_F16), FP32
- * sums, D rounded once to d_type.  The gradient of A is the same product of D's gradient
- * with the same weights in the other layout (N and K swapped).
+ * sums, D rounded once to d_type.  The sums are the tensor cores': they truncate, and a sum
+ * of K products is off by at most K * 2^-23 of the sum of their magnitudes (random values
+ * at K = 4096: 4e-6 of the result's norm, where FP32 additions rounded to nearest have 6e-7).
+ * The gradient of A is the same product of D's gradient with the same weights in the other
+ * layout (N and K swapped).
  * mpk_gemm_grouped_int8: as mpk_gemm_int8, B_scales [E][N].
  * mpk_gemm_grouped_mxfp8: A in MXFP8 (codes and scales as in the GEMM above, contiguous),
- * BF16 B [K][N], D in MXFP8 along N (contiguous).  A is dequantized exactly to BF16 into
- * a workspace of the library's pool first. */
+ * BF16 B [K][N], D in MXFP8 along N (contiguous).  A is dequantized to BF16 into a workspace
+ * of the library's pool first: as the codec does to FP32, then rounded to nearest, which is
+ * exact for scale bytes 3 to 246 (below, subnormal codes are finer than BF16's smallest step;
+ * above, values from 2^128 on are infinite in FP32 too).  A sum next to the border between
+ * two codes may take either, its error being that of the FP32 sums above. */
 int mpk_gemm_grouped(const void* A, int64_t lda, const void* B, int64_t ldb, int b_layout, int ab_type, void* D,
                      int d_type, int64_t ldd, const int32_t* offsets, int E, int M, int N, int K, void* stream);
 int mpk_gemm_grouped_int8(const int8_t* A, int64_t lda, const float* A_scales, const int8_t* B, int64_t ldb,

@@ -136,7 +136,8 @@ struct ProductArgs {
 constexpr int kTypeInt8 = 16, kTypeMxfp8 = 17;
 constexpr int kMaxGroups = 1024;
 // MXFP8 [M][K] -> BF16 rows ld_out apart (a multiple of 8; out 16-byte aligned), any K and
-// alignment; elements between K and the next multiple of 8 become zeros.
+// alignment.  Elements between K and the next multiple of 8 become the code 0's value: zero, or
+// NaN under a scale byte of 255.  The product reads none of them.
 cudaError_t launch_mxfp8_unpack_rows(const uint8_t* data, const uint8_t* scales, void* out, int64_t M, int64_t K,
                                      int64_t ld_out, cudaStream_t stream);
 // rows x cols elements of 1 or 2 bytes, rows ldx apart, to rows ld_out apart (a multiple of 16

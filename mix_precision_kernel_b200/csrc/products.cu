@@ -33,9 +33,9 @@
 // fewer tiles than SMs, the CTAs of a cluster share a tile's reduction and join their
 // sums through distributed shared memory in a fixed order (splits).
 //
-// What bounds it (B200): few rows, the weights' bytes (6.1 to 6.3 TB/s of the 6.5 a copy
-// reaches, once every SM has a tile; 16 tokens through 16 experts of 2048x2048 in 24.2 us
-// against 20.6 for the bytes alone); many rows, the tensor pipe and, over seconds, the
+// What bounds it (B200): few rows, the weights' bytes (16 tokens through 16 experts of
+// 2048x2048 BF16 in 24 us: 5.6 TB/s over the whole call, of the 6.5 a copy reaches, its launch
+// and first loads included); many rows, the tensor pipe and, over seconds, the
 // power cap (int8 4096x12288x4096 in 128 us, 3.2 POP/s, the pipe busy 82 % of the time; BF16
 // with one group 262 to 269 us, 1.53 to 1.57 PFLOP/s); a short reduction, the epilogue's
 // stores (weight gradient of 32 x 2048x2816 BF16 in 87 us, 4.2 TB/s).
