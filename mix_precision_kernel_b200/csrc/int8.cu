@@ -23,8 +23,9 @@ using namespace int8;
 // ------------------------------- rows ---------------------------------------
 // kPerRow threads hold a row in registers, up to kHold 16-byte pieces each, all loaded
 // before the first is used: one pass over x.  Longer rows are read twice, the second time
-// from L1 or L2.  16384 x 2048 BF16 in 22.2 us (4.5 TB/s of the least bytes), 4096 x 8192 FP32
-// in 34.3 us (4.9 TB/s).
+// from L1 or L2.  Captured, with other rows each time: 16384 x 2048 BF16 in 22.2 us (4.5 TB/s of
+// the least bytes), 4096 x 8192 FP32 in 34.3 us (4.9 TB/s).  Two blocks fit an SM (127 registers),
+// and a warp's loads, maximum and stores follow one another: HBM idles at each row's end.
 constexpr int kRowThreads = 256, kHold = 16;
 
 template <class D, int kPerRow>
